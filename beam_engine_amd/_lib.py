@@ -31,6 +31,7 @@ BE_PLAN_NO_WIDE256 = 1024
 BE_PLAN_NO_TAIL_ROLE = 2048
 BE_PLAN_NO_BLOCKS = 4096
 BE_PLAN_LESS_SCRATCH = 8192
+BE_PLAN_KV8 = 16384
 BE_RUN_ATTENTION, BE_RUN_MERGE = 1, 2
 BE_TEMP_RECIPROCAL, BE_TEMP_DIVIDE = 0, 1
 
@@ -102,7 +103,8 @@ EXPORTS = (
     "be_pages_release", "be_pages_reserve", "be_pages_num_free", "be_pages_ref_count", "be_pages_free_list",
     "be_trie_create", "be_trie_destroy", "be_trie_add_root", "be_trie_apply", "be_trie_sizes",
     "be_trie_candidates", "be_trie_export", "be_trie_metadata", "be_trie_plan", "be_trie_levels",
-    "be_trie_plan_kind", "be_trie_metadata_kind", "be_read_probe",
+    "be_trie_plan_kind", "be_trie_metadata_kind", "be_read_probe", "be_kv8_append", "be_kv8_rope_append",
+    "be_kv8_page_copy", "be_kv8_values", "be_attn_run_kv8",
 )
 
 _lib = None
@@ -128,6 +130,11 @@ def load() -> ctypes.CDLL:
     lib.be_kv_append.argtypes = [vp, i32, i32, i32, i32, i32, vp, vp, vp, i64, i64, vp, i64, i64, i32, vp, vp]
     lib.be_rope_qkv_append.argtypes = [vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, i32, vp, vp, i32, i32, vp, vp,
                                        vp, vp]
+    lib.be_kv8_append.argtypes = [vp, vp, i32, i32, i32, i32, i32, vp, vp, vp, i64, i64, vp, i64, i64, i32, vp, vp]
+    lib.be_kv8_rope_append.argtypes = [vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, i32, vp, vp, vp, i32, i32, vp, vp,
+                                       vp, vp]
+    lib.be_kv8_page_copy.argtypes = [vp, i64, vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, vp]
+    lib.be_kv8_values.argtypes = [vp, vp, i32, i32, i32, i32, i32, i32, vp, vp]
     lib.be_add_rms_norm.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, ctypes.c_float, vp]
     lib.be_silu_mul.argtypes = [vp, vp, i32, i32, i32, vp]
     lib.be_page_copy.argtypes = [vp, i64, i32, i32, i32, i32, i32, i32, vp, vp, vp, i32, vp, vp]
@@ -136,6 +143,8 @@ def load() -> ctypes.CDLL:
                                  ctypes.POINTER(BePlanCaps), vp, i64, ctypes.POINTER(BeAttnPlanInfo)]
     lib.be_attn_run.argtypes = [ctypes.POINTER(BeAttnPlanInfo), vp, vp, vp, i64, i64, vp, vp, i64, i64, vp,
                                 ctypes.c_float, i32, vp]
+    lib.be_attn_run_kv8.argtypes = [ctypes.POINTER(BeAttnPlanInfo), vp, vp, vp, i64, i64, vp, vp, vp, i64, i64, vp,
+                                    ctypes.c_float, i32, vp]
     lib.be_merge_states.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, i32, vp]
     lib.be_beam_topk_workspace_bytes.argtypes = [i32, i32, i32]
     lib.be_beam_topk_workspace_bytes.restype = i64
@@ -218,3 +227,21 @@ def raw_stream(t: torch.Tensor) -> int:
 def require_device(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a HIP device tensor (got {t.device}); there is no CPU path")
+
+
+class _OnCurrent:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_ON_CURRENT = _OnCurrent()
+
+
+def on_device(t: torch.Tensor):
+    """A context with ``t``'s device current, for a launch on its stream (nothing to
+    enter where it is)."""
+    dev = t.get_device()
+    return _ON_CURRENT if dev < 0 or torch._C._cuda_getDevice() == dev else torch.cuda.device(dev)

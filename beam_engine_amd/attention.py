@@ -11,6 +11,12 @@ Semantics (every level, every group): o = softmax(sm_scale * q K^T) V over the
 group's valid tokens, query head h reading KV head h // (Hq / Hkv); levels are
 merged by log-sum-exp.  ``run(..., return_lse=True)`` returns the natural-log
 lse (FlashInfer returns base 2; the reference never reads it).
+
+A cache held in 8 bits (``PageTable(store_dtype=torch.float8_e4m3fn)``): plan with
+``kv_data_type=torch.float8_e4m3fn`` beside a bf16 or fp16 ``q_data_type`` and give
+``run`` the layer's scales, ``run(q, kv_layer, kv_scale=scales)``.  K and V are then
+the values that codes and scales stand for; queries, probabilities and output keep
+the 16-bit type.  Page sizes up to 1024; not for fp32 queries.
 """
 
 from __future__ import annotations
@@ -95,7 +101,7 @@ class PlanStats:
         self.num_items = int(info.num_items)
         self.num_part_rows = int(info.num_part_rows)
         self.num_merge = int(info.num_merge)
-        self.kernel = {0: "valu", 1: "tile", 2: "stream", 3: "rows"}[int(info.kernel)]
+        self.kernel = {0: "valu", 1: "tile", 2: "stream", 3: "rows", 4: "kv8"}[int(info.kernel)]
         self.num_tails = int(info.num_tails) if self.kernel == "stream" else 0
         self.chunk_tokens = int(info.chunk_tokens)
         merge = (int(info.grid_merge) > 0 and not info.fused_merge) or int(info.grid_zero) > 0
@@ -105,7 +111,9 @@ class PlanStats:
             self.launches = ("attn_stream_kernel",) + (("tail_merge_kernel",) if info.grid_merge > 0 else ())
         else:
             rows = int(info.tile_rows)
-            if info.kernel == 0:
+            if info.kernel == 4:
+                name = "attn_kv8_kernel"
+            elif info.kernel == 0:
                 name = "attn_f32_kernel" if rows and info.dtype == _lib.dtype_code(torch.float32) else "attn_valu_kernel"
             else:
                 name = "attn_block_kernel" if rows == 128 and int(info.head_dim) <= 128 else "attn_tile_kernel"
@@ -143,12 +151,22 @@ class _PagedPlanner:
         self._no_wide256 = False      # streaming kernel: wide roles on 128-row segments only
         self._no_blocks = False       # causal groups stay on the streaming kernel where it applies
         self._rows = None             # row-block kernel: True forces it, False forbids it, None lets the planner pick
+        self._kv8 = False             # the cache holds 8 bits (kv_data_type of the last plan)
         self._num_cus: Optional[int] = None   # planner's CU count (default: the device's)
         self._caps: Optional[_lib.BePlanCaps] = None
         self._views_key = None          # (plan bytes, workspace bytes) of the cached workspace views
         self._views = (None, None)
 
     # ---------------------------------------------------------------- plan
+    def _set_kv_type(self, q_data_type, kv_data_type) -> None:
+        q, kv = (getattr(torch, t) if isinstance(t, str) else t for t in (q_data_type, kv_data_type))
+        if kv is torch.float8_e4m3fn:
+            if q not in (torch.float16, torch.bfloat16):
+                raise NotImplementedError(f"an 8-bit cache takes float16 or bfloat16 queries, not {q}")
+        elif kv is not None and kv is not q:
+            raise NotImplementedError("q and KV must share one dtype, or the cache be torch.float8_e4m3fn")
+        self._kv8 = kv is torch.float8_e4m3fn
+
     def _plan_levels(self, qo: Sequence, kvp: Sequence, kvi: Sequence, lpl: Sequence, num_qo_heads: int,
                      num_kv_heads: int, head_dim: int, page_size: int, sm_scale: Optional[float],
                      q_data_type, num_queries: Optional[int] = None, causal: bool = False) -> None:
@@ -225,7 +243,8 @@ class _PagedPlanner:
             (_lib.BE_PLAN_NO_WIDE256 if self._no_wide256 else 0) | \
             (_lib.BE_PLAN_NO_BLOCKS if self._no_blocks else 0) | \
             (_lib.BE_PLAN_ROWS if self._rows is True else 0) | \
-            (_lib.BE_PLAN_NO_ROWS if self._rows is False else 0)
+            (_lib.BE_PLAN_NO_ROWS if self._rows is False else 0) | \
+            (_lib.BE_PLAN_KV8 if self._kv8 else 0)
 
     def _install_plan(self, info, buf: torch.Tensor, staging: Optional["_Staging"], max_page: int, head_dim: int,
                       sm_scale: Optional[float], q_data_type, upload: bool = True) -> None:
@@ -262,11 +281,15 @@ class _PagedPlanner:
 
     # ---------------------------------------------------------------- run
     def _run(self, q: torch.Tensor, kv: torch.Tensor, out: Optional[torch.Tensor], return_lse: bool,
-             between=None):
+             between=None, kv_scale: Optional[torch.Tensor] = None):
         info = self._info
         if info is None:
             raise RuntimeError("plan() must be called before run()")
         lib = _lib.load()
+        kv8 = info.kernel == 4
+        if kv8 is (kv_scale is None):
+            raise ValueError("the plan is of an 8-bit cache: run() needs kv_scale" if kv8 else
+                             "kv_scale belongs to plans with kv_data_type=torch.float8_e4m3fn")
         _lib.require_device(q, "q")
         _lib.require_device(kv, "paged_kv_cache")
         # a decode step's smallest layers take about 10 us on the GPU: this call's
@@ -285,7 +308,18 @@ class _PagedPlanner:
             raise ValueError("paged_kv_cache must be contiguous")
         if ks[0] <= self._max_page:
             raise ValueError(f"plan references page {self._max_page}, cache has {ks[0]} pages")
-        if q.dtype != dt or kv.dtype != dt:
+        if kv8:
+            if q.dtype != dt or kv.dtype is not torch.float8_e4m3fn:
+                raise ValueError(f"q ({q.dtype}) must match the planned dtype {dt}, the cache ({kv.dtype}) be float8_e4m3fn")
+            if kv_scale.dtype is not torch.float8_e8m0fnu or kv_scale.shape != (ks[0], 2, hkv) or \
+                    not kv_scale.is_contiguous():
+                raise ValueError(f"kv_scale must be a contiguous [{ks[0]}, 2, {hkv}] tensor of float8_e8m0fnu, got "
+                                 f"{tuple(kv_scale.shape)} of {kv_scale.dtype}")
+            dev = q.get_device()
+            if kv.get_device() != dev or kv_scale.get_device() != dev or self._ws.get_device() != dev or \
+                    (out is not None and out.get_device() != dev):
+                raise ValueError("q, the cache, its scales, out and the workspace must be on one device")
+        elif q.dtype != dt or kv.dtype != dt:
             raise ValueError(f"q ({q.dtype}) and cache ({kv.dtype}) must match the planned dtype {dt}")
         es = 4 if dt is torch.float32 else 2
         sn, sh, sd = q.stride()
@@ -305,9 +339,21 @@ class _PagedPlanner:
             if op % 16 or (on * es) % 16 or (oh * es) % 16:
                 raise ValueError("out must be 16-byte aligned in every row (vector stores)")
         lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if return_lse else None
+        stream = _lib.raw_stream(q)
+        if kv8:
+            args = (ctypes.byref(info), self._plan_dev.data_ptr(), _lib.ptr(self._partials), qp, sn, sh, kv.data_ptr(),
+                    kv_scale.data_ptr(), op, on, oh, _lib.ptr(lse), self._sm_scale)
+            with _lib.on_device(q):
+                if between is None:
+                    _lib.check(lib.be_attn_run_kv8(*args, _lib.BE_RUN_ATTENTION | _lib.BE_RUN_MERGE, stream),
+                               "attention run")
+                else:
+                    _lib.check(lib.be_attn_run_kv8(*args, _lib.BE_RUN_ATTENTION, stream), "attention run")
+                    between()
+                    _lib.check(lib.be_attn_run_kv8(*args, _lib.BE_RUN_MERGE, stream), "attention merge")
+            return (out, lse) if return_lse else out
         args = (ctypes.byref(info), self._plan_dev.data_ptr(), _lib.ptr(self._partials), qp, sn, sh, kv.data_ptr(), op,
                 on, oh, _lib.ptr(lse), self._sm_scale)
-        stream = _lib.raw_stream(q)
         if between is None:
             rc = lib.be_attn_run(*args, _lib.BE_RUN_ATTENTION | _lib.BE_RUN_MERGE, stream)
             if rc:
@@ -357,8 +403,7 @@ class MultiLevelCascadeAttentionWrapper(_PagedPlanner):
             raise NotImplementedError("RoPE is applied before attention (pos_encoding_mode='NONE' only)")
         if window_left not in (-1, None) or logits_soft_cap not in (None, 0.0):
             raise NotImplementedError("sliding window / soft cap are not part of the decode path")
-        if kv_data_type is not None and kv_data_type != q_data_type:
-            raise NotImplementedError("q and KV must share one dtype")
+        self._set_kv_type(q_data_type, kv_data_type)
         # causal applies to the last level: query i of a group of n sees the
         # group's first kv_len - n + i + 1 tokens; one query per group (the
         # decode case) masks nothing and keeps the streaming kernel
@@ -370,8 +415,8 @@ class MultiLevelCascadeAttentionWrapper(_PagedPlanner):
                           num_qo_heads, num_kv_heads, head_dim, page_size, sm_scale, q_data_type, causal=mask)
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
-            return_lse: bool = False, between=None):
-        return self._run(q, paged_kv_cache, out, return_lse, between)
+            return_lse: bool = False, between=None, kv_scale: Optional[torch.Tensor] = None):
+        return self._run(q, paged_kv_cache, out, return_lse, between, kv_scale)
 
     forward = run
 
@@ -389,15 +434,14 @@ class BatchDecodeWithPagedKVCacheWrapper(_PagedPlanner):
              sm_scale: Optional[float] = None, **_unused) -> None:
         if pos_encoding_mode != "NONE":
             raise NotImplementedError("RoPE is applied before attention (pos_encoding_mode='NONE' only)")
-        if kv_data_type is not None and kv_data_type != q_data_type:
-            raise NotImplementedError("q and KV must share one dtype")
+        self._set_kv_type(q_data_type, kv_data_type)
         n = len(_as_i32(last_page_len))
         self._plan_levels([np.arange(n + 1, dtype=np.int32)], [indptr], [indices], [last_page_len],
                           num_qo_heads, num_kv_heads, head_dim, page_size, sm_scale, q_data_type)
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
-            return_lse: bool = False, between=None):
-        return self._run(q, paged_kv_cache, out, return_lse, between)
+            return_lse: bool = False, between=None, kv_scale: Optional[torch.Tensor] = None):
+        return self._run(q, paged_kv_cache, out, return_lse, between, kv_scale)
 
     forward = run
 
@@ -427,16 +471,15 @@ class BatchPrefillWithPagedKVCacheWrapper(_PagedPlanner):
             raise NotImplementedError("sliding window / soft cap are not supported")
         if head_dim_vo is not None and head_dim_vo != head_dim_qk:
             raise NotImplementedError("head_dim_vo must equal head_dim_qk")
-        if kv_data_type is not None and kv_data_type != q_data_type:
-            raise NotImplementedError("q and KV must share one dtype")
+        self._set_kv_type(q_data_type, kv_data_type)
         qo = _as_i32(qo_indptr)
         self._plan_levels([qo], [paged_kv_indptr], [paged_kv_indices], [paged_kv_last_page_len], num_qo_heads,
                           num_kv_heads, head_dim_qk, page_size, sm_scale, q_data_type,
                           causal=bool(causal) and len(qo) > 1 and int(np.max(np.diff(qo))) > 1)
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
-            return_lse: bool = False):
-        return self._run(q, paged_kv_cache, out, return_lse)
+            return_lse: bool = False, kv_scale: Optional[torch.Tensor] = None):
+        return self._run(q, paged_kv_cache, out, return_lse, kv_scale=kv_scale)
 
     forward = run
 

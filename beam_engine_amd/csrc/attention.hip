@@ -258,6 +258,15 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   if (d != 64 && d != 128 && d != 256) return fail(BE_ERR_UNSUPPORTED, "head_dim %d: kernels exist for 64, 128, 256", d);
   if (g > kMaxTileRows) return fail(BE_ERR_UNSUPPORTED, "GQA group %d exceeds %d", g, kMaxTileRows);
   if (num_cus <= 0) num_cus = 256;
+  // a cache held in 8 bits: dtype is that of q, the probabilities and the output
+  const bool kv8 = (flags & BE_PLAN_KV8) != 0;
+  if (kv8) {
+    if (dtype == BE_F32) return fail(BE_ERR_UNSUPPORTED, "an 8-bit cache takes fp16 / bf16 queries");
+    if (g > kMaxRowsKv8) return fail(BE_ERR_UNSUPPORTED, "GQA group %d exceeds %d (8-bit cache)", g, kMaxRowsKv8);
+    if (page_size > kMaxPageKv8) return fail(BE_ERR_UNSUPPORTED, "page size %d exceeds %d (8-bit cache)", page_size, kMaxPageKv8);
+    if (flags & (BE_PLAN_FORCE_VALU | BE_PLAN_FUSED_MERGE | BE_PLAN_ROWS))
+      return fail(BE_ERR_UNSUPPORTED, "plan flags %d: an 8-bit cache has one kernel, with a separate merge", flags);
+  }
 
   // ---- validate levels, collect groups
   std::vector<Group> groups;
@@ -318,7 +327,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
       valid[L.kv_indices[i]] = 0;
     }
   }
-  const int64_t es = (int64_t)dtype_size(dtype);
+  const int64_t es = (int64_t)dtype_size(dtype), kv_es = kv8 ? 1 : es;
   double flops = 0.0;
   // causal (BE_PLAN_CAUSAL): on the last level, query q0 + i of a group of n
   // queries sees its first kv_len - n + i + 1 tokens (FlashInfer's alignment of
@@ -350,7 +359,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   // key splits and fp32 partial rows; a 1000-token prompt, 32 / 8 heads, head_dim
   // 128, takes 9.8 MB of workspace where 32-row items take 12.5 KB)
   const bool less = (flags & BE_PLAN_LESS_SCRATCH) != 0;
-  int rows_cap = mfma ? (d == 256 ? 64 : kMaxTileRows) : f32 && !less ? 64 : kMaxRows;
+  int rows_cap = kv8 ? kMaxRowsKv8 : mfma ? (d == 256 ? 64 : kMaxTileRows) : f32 && !less ? 64 : kMaxRows;
   if (caps) {
     BE_REQUIRE(!(flags & BE_PLAN_FUSED_MERGE), "the fused merge is not available with a fixed-capacity layout");
     const int tr = caps->tile_rows;
@@ -367,7 +376,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   // merge-free row blocks (decode plans, compact layout): forced by
   // BE_PLAN_ROWS, else chosen when rows_preferred says so
   bool rows_ok = false;
-  if (!any_causal && !caps && stream_eligible(dtype, d, g, page_size, flags) && g <= 16 &&
+  if (!kv8 && !any_causal && !caps && stream_eligible(dtype, d, g, page_size, flags) && g <= 16 &&
       !(flags & BE_PLAN_NO_ROWS) && ((flags & BE_PLAN_ROWS) || rows_preferred(groups, num_queries, g, num_cus))) {
     memset(info, 0, sizeof(*info));
     const int rc = rows_plan(groups, levels, num_levels, total_pages, num_queries, hq, hkv, page_size, num_cus, out,
@@ -442,7 +451,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   // causal groups of enough query rows run as 128-row blocks rather than on the
   // streaming kernel, unless its even shares of the same tiles and its merge of
   // 16-bit slots take less
-  const bool streams = stream_eligible(dtype, d, g, page_size, flags);
+  const bool streams = !kv8 && stream_eligible(dtype, d, g, page_size, flags);
   const bool blocks = streams && !caps && !less && !(flags & BE_PLAN_NO_BLOCKS) && causal_blocks >= kMinCausalBlocks &&
                       block_us <= kStreamUs + kStreamTileUs * tiles / num_cus + kStreamRowUs * queries * hq +
                                       kStreamSpanUs * span / kTile;
@@ -616,9 +625,9 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   info->page_size = page_size;
   info->num_pages = num_pages;
   info->dtype = dtype;
-  info->kernel = blocks ? 2 : mfma ? 1 : 0;
+  info->kernel = kv8 ? 4 : blocks ? 2 : mfma ? 1 : 0;
   info->stream_loop = blocks ? kLoopBlocks : 0;
-  info->tile_rows = !mfma && !f32 ? 0 : blocks ? 128 : caps ? (f32 ? rows_cap : caps->tile_rows) : (max_r <= 16 ? 16 : max_r <= 32 ? 32 : max_r <= 64 ? 64 : 128);
+  info->tile_rows = !mfma && !f32 ? 0 : blocks ? 128 : caps ? (f32 || kv8 ? rows_cap : caps->tile_rows) : (max_r <= 16 ? 16 : max_r <= 32 ? 32 : max_r <= 64 ? 64 : 128);
   info->chunk_tokens = (int32_t)std::min<int64_t>(causal_chunk > 0 ? std::min(causal_chunk, chunk_cap) : chunk, INT32_MAX);
   info->plan_ints = (int32_t)off;
   info->off_items = (int32_t)off_items;
@@ -640,7 +649,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   info->counter_offset = ceil_div((int64_t)info->part_rows_cap * hq * (d + 1) * 4, 256) * 256;
   info->counter_bytes = info->fused_merge ? (int64_t)merge_q.size() * hkv * 4 : 0;
   info->partial_bytes = info->counter_offset + info->counter_bytes;
-  info->kv_bytes = valid_tokens * hkv * d * es * 2;
+  info->kv_bytes = valid_tokens * hkv * d * kv_es * 2;
   info->qo_bytes = (int64_t)num_queries * hq * d * es * 2;
   info->flops = flops;
   return BE_OK;
@@ -696,15 +705,17 @@ static int launch_merge(const be_attn_plan_info* info, MergeArgs& m, int count, 
 }
 
 int attn_run(const be_attn_plan_info* info, const int32_t* plan, void* partials, const void* q,
-             int64_t q_sn, int64_t q_sh, const void* kv, void* out, int64_t o_sn, int64_t o_sh,
+             int64_t q_sn, int64_t q_sh, const void* kv, const uint8_t* kv_scale, void* out, int64_t o_sn, int64_t o_sh,
              float* lse, float sm_scale, int phases, void* stream) {
   BE_REQUIRE(phases >= 1 && phases <= 3, "phases must be a non-empty subset of attention | merge");
   BE_REQUIRE(info && plan, "null plan");
   BE_REQUIRE(q && kv && out, "null q / kv / out");
+  BE_REQUIRE((info->kernel == 4) == (kv_scale != nullptr), info->kernel == 4 ? "the plan is of an 8-bit cache: scales are needed"
+                                                                             : "the plan is not of an 8-bit cache");
   BE_REQUIRE(info->part_rows_cap == 0 || partials, "plan needs %lld bytes of partial scratch", (long long)info->partial_bytes);
   BE_REQUIRE(info->num_qo_heads % info->num_kv_heads == 0, "corrupt plan info");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const bool worklist = info->kernel < 2 || (info->kernel == 2 && info->stream_loop == kLoopBlocks);
+  const bool worklist = info->kernel < 2 || info->kernel == 4 || (info->kernel == 2 && info->stream_loop == kLoopBlocks);
   BE_REQUIRE(worklist || (reinterpret_cast<uintptr_t>(kv) & 15) == 0, "the cache must be 16-byte aligned");
   if (info->kernel == 2 && info->stream_loop != kLoopBlocks)
     return stream_run(info, plan, partials, q, q_sn, q_sh, kv, out, o_sn, o_sh, lse, sm_scale, phases, st);
@@ -712,7 +723,7 @@ int attn_run(const be_attn_plan_info* info, const int32_t* plan, void* partials,
   const int64_t rows = info->part_rows_cap;
   AttnArgs a;
   a.q = q; a.q_sn = q_sn; a.q_sh = q_sh;
-  a.kv = kv; a.out = out; a.o_sn = o_sn; a.o_sh = o_sh; a.out_lse = lse;
+  a.kv = kv; a.kv_scale = kv_scale; a.out = out; a.o_sn = o_sn; a.o_sh = o_sh; a.out_lse = lse;
   a.part_o = reinterpret_cast<float*>(partials);
   a.part_lse = a.part_o + rows * info->num_qo_heads * info->head_dim;
   a.items = reinterpret_cast<const WorkItem*>(plan + info->off_items);
@@ -731,8 +742,10 @@ int attn_run(const be_attn_plan_info* info, const int32_t* plan, void* partials,
                    ? reinterpret_cast<int32_t*>(reinterpret_cast<char*>(partials) + info->counter_offset)
                    : nullptr;
   int rc = BE_OK;
+  if (info->kernel == 4) BE_REQUIRE(rows_aligned(info, a), "rows of q, out and an 8-bit cache must start on 16 bytes");
   if ((phases & BE_RUN_ATTENTION) && info->grid_items > 0) {
-    switch (info->dtype) {
+    if (info->kernel == 4) rc = kv8_launch(info, a, st);
+    else switch (info->dtype) {
       case BE_F32: rc = launch_attn<float>(info, a, st); break;
       case BE_F16: rc = launch_attn<f16_t>(info, a, st); break;
       case BE_BF16: rc = launch_attn<bf16_t>(info, a, st); break;
@@ -777,8 +790,16 @@ int be_attn_plan(const be_level* levels, int num_levels, int num_queries, int nu
 int be_attn_run(const be_attn_plan_info* info, const int32_t* dev_plan, void* partials, const void* q,
                 int64_t q_stride_n, int64_t q_stride_h, const void* kv_layer, void* out, int64_t o_stride_n,
                 int64_t o_stride_h, float* lse, float sm_scale, int phases, void* stream) {
-  return be::attn_run(info, dev_plan, partials, q, q_stride_n, q_stride_h, kv_layer, out, o_stride_n,
+  return be::attn_run(info, dev_plan, partials, q, q_stride_n, q_stride_h, kv_layer, nullptr, out, o_stride_n,
                       o_stride_h, lse, sm_scale, phases, stream);
+}
+
+int be_attn_run_kv8(const be_attn_plan_info* info, const int32_t* dev_plan, void* partials, const void* q,
+                    int64_t q_stride_n, int64_t q_stride_h, const void* kv_layer, const void* scale_layer, void* out,
+                    int64_t o_stride_n, int64_t o_stride_h, float* lse, float sm_scale, int phases, void* stream) {
+  BE_REQUIRE(scale_layer, "null scales");
+  return be::attn_run(info, dev_plan, partials, q, q_stride_n, q_stride_h, kv_layer, static_cast<const uint8_t*>(scale_layer),
+                      out, o_stride_n, o_stride_h, lse, sm_scale, phases, stream);
 }
 
 int be_merge_states(const float* o_a, const float* lse_a, const float* o_b, const float* lse_b, float* o_out,

@@ -39,6 +39,7 @@ struct AttnArgs {
   const void* q;
   int64_t q_sn, q_sh;
   const void* kv;
+  const uint8_t* kv_scale;     // 8-bit caches: e8m0 bytes [P, 2, Hkv]
   void* out;
   int64_t o_sn, o_sh;
   float* out_lse;
@@ -256,6 +257,12 @@ int tile_launch(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st
 // Launches the fp32 kernel (attn_f32.hip) over a work list whose items hold up to
 // 64 rows: one workgroup per (item, KV head).
 int f32_launch(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st);
+
+// Launches the 8-bit cache's kernel (attn_kv8.hip) over a work list: one workgroup
+// per (item, KV head).
+int kv8_launch(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st);
+constexpr int kMaxPageKv8 = 1024;      // tokens of a page of an 8-bit cache
+constexpr int kMaxRowsKv8 = 64;        // rows of its items
 
 // ---------------------------------------------------------------- 128-row blocks (attn_block.hip)
 // A streaming plan's stream_loop when its causal groups run as 128-row blocks.

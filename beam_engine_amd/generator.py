@@ -82,6 +82,8 @@ class BatchedBeamSearch:
         self.include_self = include_self or kernel_type == "fasttree"
         self.eos_token_id = eos_token_id    # a pick of this token finishes its beam (off: None)
         self.device = page_table.device
+        # an 8-bit cache: the attention plans name its type, and each layer's run its scales
+        self._kv_type = page_table.store_dtype if page_table.kv8 else None
         # the trie and its pages live in native code: one call per selection,
         # one for the step's metadata and attention plan (any strategy kind)
         self.state = NativeBeamState(beam_size, page_table)
@@ -179,7 +181,7 @@ class BatchedBeamSearch:
         w = MultiLevelCascadeAttentionWrapper(len(levels), self.ws)
         w.plan([l[0] for l in levels], [l[1] for l in levels], [l[2] for l in levels], [l[3] for l in levels],
                cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, self.pt.page_size,
-               causal=causal, q_data_type=m.dtype)
+               causal=causal, q_data_type=m.dtype, kv_data_type=self._kv_type)
         self.last_attn = w
         return w
 
@@ -207,7 +209,7 @@ class BatchedBeamSearch:
         if w is not None:
             w.num_levels = len(levels)
             try:
-                w.plan(*args, causal=causal, q_data_type=m.dtype)
+                w.plan(*args, causal=causal, q_data_type=m.dtype, kv_data_type=self._kv_type)
             except MemoryError:
                 w = None                            # outgrew the layout: re-size below
             else:
@@ -216,16 +218,19 @@ class BatchedBeamSearch:
                 return None
         # size the layout: this step's compact plan, doubled, with margins
         probe = MultiLevelCascadeAttentionWrapper(len(levels), self.ws)
-        probe.plan(*args, causal=causal, q_data_type=m.dtype)
+        probe.plan(*args, causal=causal, q_data_type=m.dtype, kv_data_type=self._kv_type)
         pi = probe._info
-        if pi.kernel != 2 or cfg.head_dim != 128:
-            self.step_graph = False                 # the fixed layout serves the streaming kernel only
+        if pi.kernel != 4 and (pi.kernel != 2 or cfg.head_dim != 128):
+            self.step_graph = False                 # the fixed layout serves the streaming kernel and 8-bit caches
             return None
         pages = sum(len(l[2]) for l in levels)
         old = self._fixed_caps
         grow = 2 if old is None else 4
-        caps = dict(max_items=grow * pi.num_items + 1024, max_queries=n,
-                    max_pages=grow * pages + 4096, max_merge=n * cfg.num_key_value_heads,
+        # (a work list launches a workgroup for every item of the layout and KV head, and
+        # one merge entry a query; the streaming kernel one record a query and KV head)
+        listed = pi.kernel == 4
+        caps = dict(max_items=grow * pi.num_items + (64 if listed else 1024), max_queries=n,
+                    max_pages=grow * pages + 4096, max_merge=n if listed else n * cfg.num_key_value_heads,
                     max_merge_rows=grow * pi.num_part_rows + 1024, max_zero=n, tile_rows=64,
                     max_tails=grow * pi.num_tails + 4096)
         if old is not None:
@@ -241,15 +246,16 @@ class BatchedBeamSearch:
             else:
                 self.pt.enable_staged_copies(2 * n)
         try:
-            w.plan(*args, causal=causal, q_data_type=m.dtype)
+            w.plan(*args, causal=causal, q_data_type=m.dtype, kv_data_type=self._kv_type)
         except (MemoryError, ValueError):
             self.step_graph = False
             return None
-        if w._info.kernel != 2:
+        if w._info.kernel not in (2, 4):
             self.step_graph = False
             return None
         self._fixed, self._fixed_caps, self._fixed_key = w, caps, self._launch_key(w._info)
-        self._gd.capture_step(lambda l, q, kv, out: w.run(q, kv, out=out))
+        scale = self.pt.kv_scale_at_layer
+        self._gd.capture_step(lambda l, q, kv, out: w.run(q, kv, out=out, kv_scale=scale[l]))
         return w
 
     @torch.no_grad()
@@ -312,11 +318,12 @@ class BatchedBeamSearch:
             tok, wpg, wps, psn = dev[0], dev[1].to(torch.int32), dev[2].to(torch.int32), dev[3]
 
         timer = self.attn_timer
+        scale = self.pt.kv_scale_at_layer
 
         def attn(li, q, kv, out=None):
             if timer is None:
-                return w.run(q, kv, out=out)
-            return timer(li, lambda between: w.run(q, kv, out=out, between=between), w)
+                return w.run(q, kv, out=out, kv_scale=scale[li])
+            return timer(li, lambda between: w.run(q, kv, out=out, between=between, kv_scale=scale[li]), w)
 
         if self.step_graphed:
             logits = self._gd.run_step()     # the staged fork copies first, inside the graph

@@ -178,7 +178,7 @@ class LlamaDecoder:
         pre = BatchPrefillWithPagedKVCacheWrapper(ws)
         pre.plan([i * s for i in range(r + 1)], [i * npg for i in range(r + 1)],
                  [p[j] for p in page_ids for j in range(npg)], [s - (npg - 1) * ps] * r, hq, hkv, d, ps,
-                 causal=True, q_data_type=self.dtype)
+                 causal=True, q_data_type=self.dtype, kv_data_type=page_table.store_dtype if page_table.kv8 else None)
         x, y = F.embedding(input_ids, self.embed), None
         for li, layer in enumerate(self.layers):
             x, h = self._add_rms(x, y, layer["ln1"])
@@ -194,7 +194,8 @@ class LlamaDecoder:
                 k = self._rope(k, pos)
                 page_table.write_blocks_vectorized(li, pages, k.reshape(r * s, hkv, d).contiguous(),
                                                    v.reshape(r * s, hkv, d).contiguous(), slots)
-            o = pre.run(q.reshape(r * s, hq, d), page_table.kv_cache_at_layer[li]).reshape(r, s, hq * d)
+            o = pre.run(q.reshape(r * s, hq, d), page_table.kv_cache_at_layer[li],
+                        kv_scale=page_table.kv_scale_at_layer[li]).reshape(r, s, hq * d)
             x, h = self._add_rms(x, F.linear(o, layer["wo"]), layer["ln2"])
             y = self._mlp(layer, h)
         last = self._rms(x[:, -1] if y is None else x[:, -1] + y[:, -1], self.norm)

@@ -19,6 +19,16 @@ Same constructor, attributes and methods.  MI355X-first differences:
 * ``copy_block`` can defer the data copy (``defer_copies()`` context) so that
   all forks of a decode step are copied in a single launch; page ids are
   allocated immediately, in the reference's order.
+* ``store_dtype=torch.float8_e4m3fn`` holds the cache in 8 bits: ``kv_pool`` are
+  e4m3 codes and ``kv_scale`` ``[L, P, 2, Hkv]`` (e8m0) the power-of-two scale of
+  each block -- the tokens of one page, K or V, one head.  Writes take and reads
+  give ``compute_dtype`` (bf16 or fp16); the writes quantise.  A page is written
+  from its first slot on: a call that writes slot 0 starts the page's blocks anew,
+  any other lets their scales grow where it has to (the earlier tokens' codes are
+  rescaled with them), and slots behind the last one written hold nothing.  Within
+  a call the entries may come in any order; the last one of a (page, slot) is kept.
+  Infinities and NaN are stored as NaN.  head_dim 64, 128 or 256, pages of up to
+  1024 tokens.
 """
 
 from __future__ import annotations
@@ -46,7 +56,19 @@ class PageCopyError(ValueError, TypeError):
 class PageTable:
     def __init__(self, layer_num: int, page_size: int = 8, max_num_pages: int = 1024, head_num: int = 32,
                  head_dim: int = 128, v_head_dim: Optional[int] = None, device: torch.device = None,
-                 store_dtype: torch.dtype = torch.float16):
+                 store_dtype: torch.dtype = torch.float16, compute_dtype: Optional[torch.dtype] = None):
+        self.kv8 = store_dtype is torch.float8_e4m3fn
+        if self.kv8:
+            compute_dtype = compute_dtype or torch.bfloat16
+            if compute_dtype not in (torch.float16, torch.bfloat16):
+                raise NotImplementedError(f"an 8-bit cache takes float16 or bfloat16 rows, not {compute_dtype}")
+            if head_dim not in (64, 128, 256):
+                raise NotImplementedError(f"an 8-bit cache: head_dim {head_dim}, kernels exist for 64, 128, 256")
+            if page_size > 1024:
+                raise NotImplementedError(f"an 8-bit cache: page size {page_size} exceeds 1024")
+        elif compute_dtype not in (None, store_dtype):
+            raise ValueError(f"compute_dtype {compute_dtype} differs from the storage dtype {store_dtype}")
+        self.compute_dtype = compute_dtype or store_dtype      # of the rows written and read back
         if v_head_dim is not None and v_head_dim != head_dim:
             raise ValueError("the paged layout stores K and V with one head_dim")
         self.layer_num = layer_num
@@ -80,6 +102,13 @@ class PageTable:
         self.kv_pool = torch.zeros((layer_num, max_num_pages, 2, page_size, head_num, head_dim),
                                    dtype=store_dtype, device=self.device)
         self.kv_cache_at_layer: List[torch.Tensor] = [self.kv_pool[l] for l in range(layer_num)]
+        # scales of an 8-bit cache (torch.zeros: 2^-127, under which code 0 stands for 0)
+        self.kv_scale: Optional[torch.Tensor] = None
+        if self.kv8:
+            self.kv_scale = torch.zeros((layer_num, max_num_pages, 2, head_num), dtype=torch.uint8,
+                                        device=self.device).view(torch.float8_e8m0fnu)
+        self.kv_scale_at_layer: List[Optional[torch.Tensor]] = [
+            self.kv_scale[l] if self.kv8 else None for l in range(layer_num)]
         self.layer_stride_bytes = self.kv_pool.stride(0) * self.kv_pool.element_size()
         # device count of append / copy entries the kernels skipped for naming a
         # page, slot or position outside the pool (read by check_errors)
@@ -223,12 +252,24 @@ class PageTable:
         else:
             dev = torch.from_numpy(np.ascontiguousarray(np.asarray(todo, dtype=np.int32).T))
         lib = _lib.load()
+        if self.kv8:
+            self._copy_kv8(dev[0].data_ptr(), dev[1].data_ptr(), dev[2].data_ptr(), 0, len(todo), "page copy")
+            return len(todo)
         rc = lib.be_page_copy(self.kv_pool.data_ptr(), self.layer_stride_bytes, self.layer_num,
                               _lib.dtype_code(self.store_dtype), self.max_num_pages, self.page_size,
                               self.head_num, self.head_dim, dev[0].data_ptr(), dev[1].data_ptr(),
                               dev[2].data_ptr(), len(todo), self._err.data_ptr(), _lib.stream_ptr(self.device))
         _lib.check(rc, "page copy")
         return len(todo)
+
+    def _copy_kv8(self, src: int, dst: int, length: int, count: int, n: int, what: str) -> None:
+        """Fork copies of codes and scales (device arrays; ``count`` 0 or the device count)."""
+        with _lib.on_device(self.kv_pool):
+            rc = self._lib.be_kv8_page_copy(self.kv_pool.data_ptr(), self.layer_stride_bytes, self.kv_scale.data_ptr(),
+                                            self.kv_scale.stride(0), self.layer_num, self.max_num_pages, self.page_size,
+                                            self.head_num, self.head_dim, src, dst, length, count, n,
+                                            self._err.data_ptr(), _lib.stream_ptr(self.device))
+        _lib.check(rc, what)
 
     # ------------------------------------------------------------ staged copies
     def enable_staged_copies(self, max_copies: int, dev: Optional[torch.Tensor] = None,
@@ -310,6 +351,9 @@ class PageTable:
         d = self._staged_dev
         m = self._staged_max
         base = d.data_ptr()
+        if self.kv8:
+            self._copy_kv8(base + 4, base + 4 * (1 + m), base + 4 * (1 + 2 * m), base, m, "staged page copy")
+            return
         rc = lib.be_page_copy_counted(self.kv_pool.data_ptr(), self.layer_stride_bytes, self.layer_num,
                                       _lib.dtype_code(self.store_dtype), self.max_num_pages, self.page_size,
                                       self.head_num, self.head_dim, base + 4, base + 4 * (1 + m),
@@ -341,7 +385,10 @@ class PageTable:
         if index > self.page_size:
             raise ValueError(f"Index {index} exceeds page size {self.page_size}")
         n = key.shape[0]
-        if n > 0:
+        if n > 0 and self.kv8:
+            slots = torch.arange(index, index + n, dtype=torch.int32, device=self.device)
+            self.write_blocks_vectorized(layer, torch.full_like(slots, page_idx), key, value, slots)
+        elif n > 0:
             self.kv_cache_at_layer[layer][page_idx, 0, index:index + n] = key
             self.kv_cache_at_layer[layer][page_idx, 1, index:index + n] = value
 
@@ -359,8 +406,8 @@ class PageTable:
         n = keys.shape[0]
         if keys.shape != values.shape or keys.dim() != 3 or keys.shape[1:] != (self.head_num, self.head_dim):
             raise ValueError(f"keys/values must be [N, {self.head_num}, {self.head_dim}]")
-        if keys.dtype != self.store_dtype or values.dtype != self.store_dtype:
-            raise ValueError(f"keys/values must be {self.store_dtype}")
+        if keys.dtype != self.compute_dtype or values.dtype != self.compute_dtype:
+            raise ValueError(f"keys/values must be {self.compute_dtype}")
         if keys.stride(2) != 1 or values.stride(2) != 1:
             keys, values = keys.contiguous(), values.contiguous()
         for t, nm in ((page_indices, "page_indices"), (indices, "indices"), (keys, "keys")):
@@ -369,6 +416,9 @@ class PageTable:
         indices = indices.to(torch.int32)
         if page_indices.numel() < n or indices.numel() < n:
             raise ValueError("page_indices / indices shorter than keys")
+        if self.kv8:
+            self._append_kv8(layer, page_indices, keys, values, indices, n)
+            return
         lib = _lib.load()
         rc = lib.be_kv_append(self.kv_cache_at_layer[layer].data_ptr(), _lib.dtype_code(self.store_dtype),
                               self.max_num_pages, self.page_size, self.head_num, self.head_dim,
@@ -377,21 +427,44 @@ class PageTable:
                               self._err.data_ptr(), _lib.stream_ptr(self.device))
         _lib.check(rc, "kv append")
 
+    def _append_kv8(self, layer: int, pages: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                    slots: torch.Tensor, n: int) -> None:
+        self._same_device((pages, "page_indices"), (slots, "indices"), (keys, "keys"), (values, "values"))
+        pages, slots = pages.reshape(-1).contiguous(), slots.reshape(-1).contiguous()
+        keys, values = (t if t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 else
+                        t.clone(memory_format=torch.contiguous_format) for t in (keys, values))
+        with _lib.on_device(self.kv_pool):
+            rc = self._lib.be_kv8_append(self.kv_cache_at_layer[layer].data_ptr(), self.kv_scale_at_layer[layer].data_ptr(),
+                                         _lib.dtype_code(self.compute_dtype), self.max_num_pages, self.page_size,
+                                         self.head_num, self.head_dim, pages.data_ptr(), slots.data_ptr(),
+                                         keys.data_ptr(), keys.stride(0), keys.stride(1), values.data_ptr(),
+                                         values.stride(0), values.stride(1), n, self._err.data_ptr(),
+                                         _lib.stream_ptr(self.device))
+        _lib.check(rc, "kv append")
+
+    def _same_device(self, *tensors) -> None:
+        for t, nm in tensors:
+            if t.get_device() != self.kv_pool.get_device():
+                raise ValueError(f"{nm} is on {t.device}, the cache on {self.kv_pool.device}")
+
     def write_rope_qkv(self, layer: int, qkv: torch.Tensor, num_qo_heads: int, positions: torch.Tensor,
                        cos: torch.Tensor, sin: torch.Tensor, page_indices: torch.Tensor, indices: torch.Tensor,
                        q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Decode-step RoPE fused with the append: ``qkv [N, (Hq + 2 Hkv) * D]``
         (q | k | v heads), ``positions [N]`` int64, HF cos/sin tables ``[max_pos, D]``.
         Writes RoPE(k) and v to ``(page_indices[i], indices[i])`` and returns
-        RoPE(q) as ``[N, Hq, D]``."""
+        RoPE(q) as ``[N, Hq, D]``.  An 8-bit cache rotates in fp32 and rounds once,
+        q to ``compute_dtype`` and k to its code; other caches round as the eager
+        tensor code does."""
         if layer < 0 or layer >= self.layer_num:
             raise ValueError(f"Layer {layer} out of range (max: {self.layer_num - 1})")
         n = qkv.shape[0]
         width = (num_qo_heads + 2 * self.head_num) * self.head_dim
         if qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
             raise ValueError(f"qkv must be [N, {width}] with a contiguous last dim")
-        if qkv.dtype != self.store_dtype or cos.dtype != self.store_dtype or sin.dtype != self.store_dtype:
-            raise ValueError(f"qkv and cos/sin tables must be {self.store_dtype}")
+        dt = self.compute_dtype
+        if qkv.dtype != dt or cos.dtype != dt or sin.dtype != dt:
+            raise ValueError(f"qkv and cos/sin tables must be {dt}")
         if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != self.head_dim or not cos.is_contiguous() \
                 or not sin.is_contiguous():
             raise ValueError("cos/sin must be contiguous [max_pos, head_dim]")
@@ -405,6 +478,8 @@ class PageTable:
             q_out = torch.empty((n, num_qo_heads, self.head_dim), dtype=qkv.dtype, device=qkv.device)
         elif q_out.shape != (n, num_qo_heads, self.head_dim) or not q_out.is_contiguous() or q_out.dtype != qkv.dtype:
             raise ValueError("q_out must be a contiguous [N, Hq, D] tensor of the storage dtype")
+        if self.kv8:
+            return self._rope_kv8(layer, qkv, num_qo_heads, positions, cos, sin, page_indices, indices, q_out, n)
         lib = _lib.load()
         rc = lib.be_rope_qkv_append(qkv.data_ptr(), qkv.stride(0), _lib.dtype_code(self.store_dtype), n, num_qo_heads,
                                     self.head_num, self.head_dim, positions.data_ptr(), cos.data_ptr(),
@@ -415,13 +490,59 @@ class PageTable:
         _lib.check(rc, "rope append")
         return q_out
 
+    def _rope_kv8(self, layer: int, qkv: torch.Tensor, hq: int, positions: torch.Tensor, cos: torch.Tensor,
+                  sin: torch.Tensor, pages: torch.Tensor, slots: torch.Tensor, q_out: torch.Tensor, n: int) -> torch.Tensor:
+        self._same_device((qkv, "qkv"), (positions, "positions"), (cos, "cos"), (sin, "sin"), (pages, "page_indices"),
+                          (slots, "indices"), (q_out, "q_out"))
+        positions, pages, slots = (t if t.is_contiguous() else t.reshape(-1).contiguous() for t in (positions, pages, slots))
+        if qkv.data_ptr() % 16 or qkv.stride(0) % 8:
+            qkv = qkv.clone(memory_format=torch.contiguous_format)
+        cos, sin = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (cos, sin))
+        if n and q_out.data_ptr() % 16:
+            raise ValueError("q_out must be 16-byte aligned")
+        with _lib.on_device(self.kv_pool):
+            rc = self._lib.be_kv8_rope_append(qkv.data_ptr(), qkv.stride(0), _lib.dtype_code(self.compute_dtype), n, hq,
+                                              self.head_num, self.head_dim, positions.data_ptr(), cos.data_ptr(),
+                                              sin.data_ptr(), cos.shape[0], q_out.data_ptr(),
+                                              self.kv_cache_at_layer[layer].data_ptr(),
+                                              self.kv_scale_at_layer[layer].data_ptr(), self.max_num_pages, self.page_size,
+                                              pages.data_ptr(), slots.data_ptr(), self._err.data_ptr(),
+                                              _lib.stream_ptr(self.device))
+        _lib.check(rc, "rope append")
+        return q_out
+
     # ------------------------------------------------------------ flat views
     def get_k_buffer(self, layer: int) -> torch.Tensor:
         """K of every slot as ``[P * page, Hkv, D]`` (a copy, as in the reference,
         page_table.py:211-226; the HIP attention path never needs it)."""
+        if self.kv8:
+            return self._values(self.kv_cache_at_layer[layer], self.kv_scale_at_layer[layer], 0)
         return self.kv_cache_at_layer[layer][:, 0].reshape(self.max_num_pages * self.page_size,
                                                            self.head_num, self.head_dim)
 
     def get_v_buffer(self, layer: int) -> torch.Tensor:
+        if self.kv8:
+            return self._values(self.kv_cache_at_layer[layer], self.kv_scale_at_layer[layer], 1)
         return self.kv_cache_at_layer[layer][:, 1].reshape(self.max_num_pages * self.page_size,
                                                            self.head_num, self.head_dim)
+
+    def dequantized(self, layer: Optional[int] = None) -> torch.Tensor:
+        """The values of an 8-bit cache in ``compute_dtype``, laid out as the codes:
+        ``[P, 2, page, Hkv, D]`` of a layer, or ``[L, P, 2, page, Hkv, D]`` of all."""
+        if not self.kv8:
+            raise ValueError("the cache is not held in 8 bits")
+        if layer is None:
+            return self._values(self.kv_pool, self.kv_scale, -1)
+        return self._values(self.kv_cache_at_layer[layer], self.kv_scale_at_layer[layer], -1)
+
+    def _values(self, codes: torch.Tensor, scale: torch.Tensor, which: int) -> torch.Tensor:
+        pages = codes.numel() // (2 * self.page_size * self.head_num * self.head_dim)
+        out = torch.empty(codes.shape if which < 0 else (pages * self.page_size, self.head_num, self.head_dim),
+                          dtype=self.compute_dtype, device=self.device)
+        _lib.require_device(codes, "the cache")
+        with _lib.on_device(codes):
+            rc = self._lib.be_kv8_values(codes.data_ptr(), scale.data_ptr(), _lib.dtype_code(self.compute_dtype), pages,
+                                         self.page_size, self.head_num, self.head_dim, which, out.data_ptr(),
+                                         _lib.stream_ptr(self.device))
+        _lib.check(rc, "dequantise")
+        return out

@@ -129,6 +129,52 @@ int be_rope_qkv_append(const void* qkv, int64_t qkv_stride_n, int dtype, int n, 
                        void* kv_layer, int num_pages, int page_size, const int32_t* page_idx,
                        const int32_t* slot, int32_t* err_count, void* stream);
 
+/* ------------------------------------------------------------------ 8-bit KV cache
+ * A layer is e4m3 codes [num_pages, 2, page_size, num_kv_heads, head_dim] and, for
+ * each block (the tokens of one page, K or V, one head), a power-of-two scale as an
+ * e8m0 byte [num_pages, 2, num_kv_heads]: a code c stands for c * 2^(byte - 127).
+ * head_dim 64, 128 or 256; the rows written and read back are fp16 or bf16 (dtype).
+ * No reference counterpart: the reference's cache holds the model's type.
+ *
+ * be_kv8_append: be_kv_append into such a layer (rows of k and v start on 16 bytes).
+ * A block's exponent is the least E >= -100 with amax <= 448 2^E over its finite
+ * values; values saturate at the largest e4m3 value times a power of two that dtype
+ * holds, NaN and infinities become NaN.  A page is written from its first slot on: a
+ * call that writes slot 0 starts its blocks anew, any other only lets their exponents
+ * grow and rescales the slots below the least one that it writes (rounded again, exact
+ * but for subnormal codes).  Slots behind the last one written hold nothing.  Entries
+ * may come in any order; the last of several of one (page, slot) is kept (all of them
+ * count for amax).  Entries with a page or slot outside the pool are skipped and
+ * counted in *err_count.
+ *
+ * be_kv8_rope_append: be_rope_qkv_append into such a layer, with the rotation in fp32:
+ * q_out = round(x*cos + rotate_half(x)*sin), each product and the sum rounded in fp32
+ * and the result to dtype once, k quantised from its fp32 rotation.  An entry whose
+ * position, page or slot is out of range is skipped and counted (its q row too, where
+ * the position is).
+ *
+ * be_kv8_page_copy: be_page_copy (count NULL) or be_page_copy_counted of codes, with
+ * the source's scales for every copy of at least one token.
+ *
+ * be_kv8_values: the values of num_pages pages (consecutive: any number of layers' too)
+ * as dtype: which -1 both planes, in the codes' layout; 0 / 1 K / V alone,
+ * [num_pages, page_size, num_kv_heads, head_dim]. */
+int be_kv8_append(void* kv_layer, void* scale_layer, int dtype, int num_pages, int page_size, int num_kv_heads,
+                  int head_dim, const int32_t* page_idx, const int32_t* pos, const void* k, int64_t k_stride_n,
+                  int64_t k_stride_h, const void* v, int64_t v_stride_n, int64_t v_stride_h, int n,
+                  int32_t* err_count, void* stream);
+int be_kv8_rope_append(const void* qkv, int64_t qkv_stride_n, int dtype, int n, int num_qo_heads,
+                       int num_kv_heads, int head_dim, const int64_t* positions, const void* cos_table,
+                       const void* sin_table, int max_position, void* q_out, void* kv_layer, void* scale_layer,
+                       int num_pages, int page_size, const int32_t* page_idx, const int32_t* slot,
+                       int32_t* err_count, void* stream);
+int be_kv8_page_copy(void* kv_pool, int64_t layer_stride_bytes, void* scale_pool, int64_t scale_stride_bytes,
+                     int num_layers, int num_pages, int page_size, int num_kv_heads, int head_dim,
+                     const int32_t* src, const int32_t* dst, const int32_t* len, const int32_t* count, int n,
+                     int32_t* err_count, void* stream);
+int be_kv8_values(const void* kv, const void* scale, int dtype, int num_pages, int page_size, int num_kv_heads,
+                  int head_dim, int which, void* out, void* stream);
+
 /* be_add_rms_norm: the decoder's residual add and the RMSNorm that reads it, one
  * pass over contiguous [rows, n] 16-bit tensors: sum = round(x + delta), out =
  * round(sum * rsqrt(mean(sum^2) + eps) * weight[n]) in fp32.  n: a multiple of 8
@@ -196,6 +242,11 @@ typedef struct be_level {
                                     partials) and elsewhere cut as decode groups are, fp32
                                     groups in 32-row tiles (half as many key splits)         */
 
+#define BE_PLAN_KV8 16384        /* the cache holds 8 bits (be_kv8_append); dtype is that of q and
+                                    the output; be_attn_run_kv8 runs the plan.  Page sizes up
+                                    to 1024; not with BE_PLAN_FORCE_VALU, BE_PLAN_FUSED_MERGE
+                                    or BE_PLAN_ROWS                                          */
+
 /* Fixed-capacity plan layout (for HIP-graph capture): every region of the
  * device plan sits at an offset that depends only on these capacities, the
  * live counts sit in a device header, and be_attn_run launches capacity-sized
@@ -220,7 +271,7 @@ typedef struct be_attn_plan_info {
                               1 = work list on the 16-bit MFMA tile kernel (tile_rows 128:
                               the block kernel), 2 = MFMA streaming (persistent; stream_loop 2:
                               a work list on the block kernel), 3 = MFMA row blocks (one
-                              kernel, no merge)                                    */
+                              kernel, no merge), 4 = work list over an 8-bit cache   */
   int32_t tile_rows;       /* most rows (queries x GQA group) of an item: 16, 32, 64, 128 */
   int32_t chunk_tokens;    /* split-K chunk length (fewer-row groups of non-causal plans
                               may take longer ones)                               */
@@ -457,6 +508,12 @@ int be_attn_run(const be_attn_plan_info* info, const int32_t* dev_plan, void* pa
                 const void* q, int64_t q_stride_n, int64_t q_stride_h, const void* kv_layer,
                 void* out, int64_t o_stride_n, int64_t o_stride_h, float* lse, float sm_scale,
                 int phases, void* stream);
+
+/* be_attn_run_kv8: be_attn_run of a BE_PLAN_KV8 plan, over a layer's codes and scales
+ * (be_kv8_append); rows of q, out and the cache must start on 16 bytes. */
+int be_attn_run_kv8(const be_attn_plan_info* info, const int32_t* dev_plan, void* partials, const void* q,
+                    int64_t q_stride_n, int64_t q_stride_h, const void* kv_layer, const void* scale_layer, void* out,
+                    int64_t o_stride_n, int64_t o_stride_h, float* lse, float sm_scale, int phases, void* stream);
 
 /* be_merge_states: (o, lse) <- merge((o_a, lse_a), (o_b, lse_b)) for n x heads
  * rows of head_dim; o_* are float [n, heads, D] contiguous, lse natural log.
