@@ -262,7 +262,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   const bool kv8 = (flags & BE_PLAN_KV8) != 0;
   if (kv8) {
     if (dtype == BE_F32) return fail(BE_ERR_UNSUPPORTED, "an 8-bit cache takes fp16 / bf16 queries");
-    if (g > kMaxRowsKv8) return fail(BE_ERR_UNSUPPORTED, "GQA group %d exceeds %d (8-bit cache)", g, kMaxRowsKv8);
+    if (g > kv8_max_rows(d)) return fail(BE_ERR_UNSUPPORTED, "GQA group %d exceeds %d (8-bit cache)", g, kv8_max_rows(d));
     if (page_size > kMaxPageKv8) return fail(BE_ERR_UNSUPPORTED, "page size %d exceeds %d (8-bit cache)", page_size, kMaxPageKv8);
     if (flags & (BE_PLAN_FORCE_VALU | BE_PLAN_FUSED_MERGE | BE_PLAN_ROWS))
       return fail(BE_ERR_UNSUPPORTED, "plan flags %d: an 8-bit cache has one kernel, with a separate merge", flags);
@@ -359,7 +359,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   // key splits and fp32 partial rows; a 1000-token prompt, 32 / 8 heads, head_dim
   // 128, takes 9.8 MB of workspace where 32-row items take 12.5 KB)
   const bool less = (flags & BE_PLAN_LESS_SCRATCH) != 0;
-  int rows_cap = kv8 ? kMaxRowsKv8 : mfma ? (d == 256 ? 64 : kMaxTileRows) : f32 && !less ? 64 : kMaxRows;
+  int rows_cap = kv8 ? kv8_max_rows(d) : mfma ? (d == 256 ? 64 : kMaxTileRows) : f32 && !less ? 64 : kMaxRows;
   if (caps) {
     BE_REQUIRE(!(flags & BE_PLAN_FUSED_MERGE), "the fused merge is not available with a fixed-capacity layout");
     const int tr = caps->tile_rows;
@@ -368,7 +368,8 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
     BE_REQUIRE(caps->max_items >= 0 && caps->max_queries >= num_queries && caps->max_pages >= 0 &&
                    caps->max_merge >= 0 && caps->max_merge_rows >= 0 && caps->max_zero >= 0,
                "bad plan capacities (max_queries %d < %d queries?)", caps->max_queries, num_queries);
-    if (mfma) rows_cap = std::min(rows_cap, tr);
+    // (an 8-bit cache: one kernel for every plan of the layout, unless a group needs blocks)
+    if (mfma) rows_cap = std::min(rows_cap, kv8 && g <= 64 ? std::min(tr, 64) : tr);
     // (fp32: never more items than 32-row ones, which capacities were sized for
     // whatever tile_rows said; causal ones cut their keys by their own rows)
     if (f32 && (tr <= 32 || any_causal)) rows_cap = kMaxRows;
@@ -547,6 +548,14 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   if (any_causal)
     std::stable_sort(items.begin(), items.end(), [](const WorkItem& x, const WorkItem& y) { return x.tok_count > y.tok_count; });
 
+  // an 8-bit cache: items of more than 64 rows first, which the block kernel takes
+  int block_items = 0;
+  if (kv8) {
+    auto big = [&](const WorkItem& w) { return w.q_count * g > 64; };
+    std::stable_partition(items.begin(), items.end(), big);
+    block_items = (int)std::count_if(items.begin(), items.end(), big);
+  }
+
   // ---- merge list (queries with partial rows: one of a tile whose other queries
   // have more items has a row too, if only one) and zero list (no keys)
   std::vector<int> merge_q, merge_ptr{0}, merge_rows, zero_q;
@@ -627,6 +636,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   info->dtype = dtype;
   info->kernel = kv8 ? 4 : blocks ? 2 : mfma ? 1 : 0;
   info->stream_loop = blocks ? kLoopBlocks : 0;
+  info->num_wg = kv8 ? (caps && block_items ? (int)c_items : block_items) : 0;
   info->tile_rows = !mfma && !f32 ? 0 : blocks ? 128 : caps ? (f32 || kv8 ? rows_cap : caps->tile_rows) : (max_r <= 16 ? 16 : max_r <= 32 ? 32 : max_r <= 64 ? 64 : 128);
   info->chunk_tokens = (int32_t)std::min<int64_t>(causal_chunk > 0 ? std::min(causal_chunk, chunk_cap) : chunk, INT32_MAX);
   info->plan_ints = (int32_t)off;

@@ -93,8 +93,17 @@ __device__ __forceinline__ void store_lse(const AttnArgs& a, const WorkItem& it,
   else if (a.out_lse) a.out_lse[(int64_t)a.q_index[it.q_begin + j] * a.hq + head] = lse;
 }
 
+// What a workgroup keeps in LDS.
+template <int D> struct TileShared {
+  unsigned char stage[2 * 2 * kTile * D];
+  int32_t pg[kMaxPagesLds];
+  uint16_t sc[kMaxPagesLds];           // scale bytes of the pages: K | V << 8
+  int32_t nan_tok[D];                  // per column: the first masked tile's token whose V is NaN
+  int32_t nan_any;
+};
+
 template <typename T, int D, int RT, bool PAGED4, bool QUADS>
-__global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_kv8_kernel(AttnArgs a) {
+__device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& it, TileShared<D>& sh) {
   constexpr int CPR = D / 16;                        // 16-code chunks of a row
   using Loader = TileLoader<D, PAGED4, swz<CPR>>;
   constexpr int PLANE = Loader::PLANE, STAGE = Loader::STAGE;
@@ -106,14 +115,10 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_kv8_kernel(AttnArg
   constexpr int COMB_SLOT = (MT * 64 * 4 + 2 * 64) * 4;
   static_assert(TS == 1 || 2 * COMB_SLOT <= 2 * STAGE, "combine scratch must fit");
 
-  __shared__ __attribute__((aligned(1024))) unsigned char stage[2 * STAGE];
-  __shared__ int32_t pg_lds[kMaxPagesLds];
-  __shared__ uint16_t sc_lds[kMaxPagesLds];          // scale bytes of the pages: K | V << 8
-  __shared__ int32_t nan_tok[D];                     // per column: the first masked tile's token whose V is NaN
-  __shared__ int32_t nan_any;
-  if (a.live_items && (int)blockIdx.x >= *a.live_items) return;
-
-  const WorkItem it = a.items[blockIdx.x];
+  unsigned char* stage = sh.stage;
+  int32_t* pg_lds = sh.pg;
+  uint16_t* sc_lds = sh.sc;
+  int32_t* nan_tok = sh.nan_tok;
   const int kvh = blockIdx.y;
   const int tid = threadIdx.x;
   const int w = rfl(tid >> 6), lane = tid & 63, lg = lane >> 4, lc = lane & 15;
@@ -157,7 +162,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_kv8_kernel(AttnArg
   ld.load(lds0);
   if (n_tiles > 1) ld.load(lds0 + STAGE);
   for (int i = tid; i < D; i += 256) nan_tok[i] = INT32_MAX;
-  if (tid == 0) nan_any = 0;
+  if (tid == 0) sh.nan_any = 0;
   // ---- the pages' scales (behind the first tiles' loads, which they need not precede)
   for (int i = tid; i < n_pages; i += 256) {
     const int64_t at = (int64_t)a.pages[it.page_begin + first_page + i] * 2 * a.hkv + kvh;
@@ -205,7 +210,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_kv8_kernel(AttnArg
     }
     if (unseen < min(it.tok_count, (tile + 1) * kTile)) {
       // tokens that a row must not see: their NaN would reach it by a weight of 0
-      set_nans_aside<D>(stage + st * STAGE + PLANE, tile * kTile, tid, nan_tok, &nan_any);
+      set_nans_aside<D>(stage + st * STAGE + PLANE, tile * kTile, tid, nan_tok, &sh.nan_any);
       stream::lds_sync();
     }
     const int s0 = tile * kTile + ts * NSUB * 16;      // first token of the wave's sub-tiles
@@ -331,7 +336,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_kv8_kernel(AttnArg
   if (ts == 0 && active && row < R) {
     const int head = kvh * g + hh, d0 = cs * MT * 16;
     const float inv = (l_run > 0.f) ? 1.f / l_run : 0.f;
-    if (nan_any) {
+    if (sh.nan_any) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -353,31 +358,369 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_kv8_kernel(AttnArg
   }
 }
 
-template <typename T, int D, int RT>
-static void launch_rt(const AttnArgs& a, dim3 grid, hipStream_t st) {
-  if (paged4(a.page_size, D) && a.page_size % 4 == 0) attn_kv8_kernel<T, D, RT, true, true><<<grid, 256, 0, st>>>(a);
-  else if (a.page_size % 4 == 0) attn_kv8_kernel<T, D, RT, false, true><<<grid, 256, 0, st>>>(a);
-  else attn_kv8_kernel<T, D, RT, false, false><<<grid, 256, 0, st>>>(a);
+// A workgroup takes as many row tiles as its item has: with fewer, the waves share out
+// the tokens of a row tile (and the columns) rather than idle.
+template <typename T, int D, bool PAGED4, bool QUADS>
+__global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_kv8_kernel(AttnArgs a, int first_item) {
+  __shared__ __attribute__((aligned(1024))) TileShared<D> sh;
+  const int item = first_item + (int)blockIdx.x;
+  if (a.live_items && item >= *a.live_items) return;
+  const WorkItem it = a.items[item];
+  const int R = it.q_count * a.g;
+  if (R <= 16) tile_item<T, D, 1, PAGED4, QUADS>(a, it, sh);
+  else if (R <= 32) tile_item<T, D, 2, PAGED4, QUADS>(a, it, sh);
+  else tile_item<T, D, 4, PAGED4, QUADS>(a, it, sh);
 }
 
 template <typename T, int D>
 static int launch_tile(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st) {
-  const dim3 grid(info->grid_items, info->num_kv_heads);
-  switch (info->tile_rows) {
-    case 16: launch_rt<T, D, 1>(a, grid, st); break;
-    case 32: launch_rt<T, D, 2>(a, grid, st); break;
-    case 64: launch_rt<T, D, 4>(a, grid, st); break;
-    default: return fail(BE_ERR_INVALID, "corrupt plan: tile_rows %d", info->tile_rows);
+  const int first = info->num_wg;                    // items of more than 64 rows come first
+  const dim3 grid(info->grid_items - first, info->num_kv_heads);
+  if (grid.x == 0) return BE_OK;
+  if (paged4(a.page_size, D) && a.page_size % 4 == 0) attn_kv8_kernel<T, D, true, true><<<grid, 256, 0, st>>>(a, first);
+  else if (a.page_size % 4 == 0) attn_kv8_kernel<T, D, false, true><<<grid, 256, 0, st>>>(a, first);
+  else attn_kv8_kernel<T, D, false, false><<<grid, 256, 0, st>>>(a, first);
+  BE_HIP_CHECK(hipGetLastError());
+  return BE_OK;
+}
+
+// ================================================================== 128-row blocks
+constexpr int kWaveRows = 32;
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+template <typename T> __device__ __forceinline__ v16f mfma32(v8s a, v8s b, v16f c) {
+  if constexpr (std::is_same<T, bf16_t>::value) {
+    typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+  } else {
+    typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
   }
+}
+
+// The 16-byte chunk XOR of a row of 16-bit values: any 16 consecutive rows' chunk and
+// the four rows x four chunks of a half wave's transposed V read fall on all banks.
+template <int D>
+__device__ __forceinline__ int swz16(int r) {
+  return D == 128 ? ((r & 3) << 2 | ((r >> 2) & 3)) : (((r >> 1) & 1) << 2 | ((r >> 2) & 3));
+}
+
+// The value of the lane with the other bit 5 (the other token quads of the same row).
+__device__ __forceinline__ float other_half(float x, bool sum) {
+  typedef unsigned int u2 __attribute__((ext_vector_type(2)));
+  const unsigned xb = __float_as_uint(x);
+  const u2 r = __builtin_amdgcn_permlane32_swap(xb, xb, false, false);
+  const unsigned a = r.x, b = r.y;
+  return sum ? __uint_as_float(a) + __uint_as_float(b) : fmaxf(__uint_as_float(a), __uint_as_float(b));
+}
+
+// Items of 65 to 128 rows (prompts, prefixes that many beams share), head_dim 64 or 128:
+// one workgroup of four waves, 32 rows each, over 64-token tiles, products on
+// v_mfma_f32_32x32x16.  At this many rows an operand is read by every wave, so a tile
+// is turned into 16-bit values once, on its way into LDS: each thread loads its share
+// of the next tile's codes into registers while the current one is computed, converts
+// it and writes it to the other stage; one barrier a tile.  K is converted relative to
+// the item's largest K scale, which the softmax's scale takes back.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void attn_kv8_block_kernel(AttnArgs a, int n_items) {
+  constexpr int KS = D / 16;                         // QK contraction steps
+  constexpr int MB = D / 32;                         // Oᵀ head_dim blocks
+  constexpr int RB = D * 2, PLANE = kTile * RB, STAGE = 2 * PLANE;
+  constexpr int CPR = D / 16;                        // 16-code chunks of a row
+  constexpr int NC = kTile * CPR / 256;              // K (and V) chunks of a thread
+  constexpr int CPR16 = D / 8, RPI = 64 / CPR16;     // of the 16-bit rows
+
+  __shared__ __attribute__((aligned(1024))) unsigned char stage[2 * STAGE];
+  __shared__ int32_t pg_lds[kMaxPagesLds];
+  __shared__ uint16_t sc_lds[kMaxPagesLds];
+  __shared__ int32_t nan_tok[D];
+  __shared__ int32_t nan_any, k_top;
+  // consecutive workgroups are the KV heads of one item: an XCD keeps the same heads in its L2
+  const int item = (int)blockIdx.x / a.hkv, kvh = (int)blockIdx.x - item * a.hkv;
+  if (item >= n_items || (a.live_items && item >= *a.live_items)) return;
+
+  const WorkItem it = a.items[item];
+  const int tid = threadIdx.x;
+  const int w = rfl(tid >> 6), lane = tid & 63, h = lane >> 5, lr = lane & 31;
+  const int g = a.g, R = it.q_count * g, ps = a.page_size;
+
+  // ---- the item's pages and their scales
+  const int first_page = it.tok_begin / ps;
+  const int n_pages = (it.tok_begin + it.tok_count - 1) / ps - first_page + 1;
+  const int n_tiles = (it.tok_count + kTile - 1) / kTile;
+  if (tid == 0) {
+    nan_any = 0;
+    k_top = 0;
+  }
+  for (int i = tid; i < D; i += 256) nan_tok[i] = INT32_MAX;
+  __syncthreads();
+  {
+    int top = 0;
+    for (int i = tid; i < n_pages; i += 256) {
+      const int id = a.pages[it.page_begin + first_page + i];
+      const int64_t at = (int64_t)id * 2 * a.hkv + kvh;
+      const int kb = a.kv_scale[at], vb = a.kv_scale[at + a.hkv];
+      pg_lds[i] = id;
+      sc_lds[i] = (uint16_t)(kb | vb << 8);
+      top = max(top, kb);
+    }
+    if (top > 0) atomicMax(&k_top, top);
+  }
+
+  // ---- this wave's rows: lane's row, the tokens it sees, the wave's most
+  const int row = w * kWaveRows + lr;
+  const bool wave_on = w * kWaveRows < R;
+  const float inv_g = 1.f / (float)g;
+  // row / g for row < 256 (the quotient's distance from an integer is at least 1 / (2 g))
+  auto query_of = [&](int r) { return (int)(((float)r + 0.5f) * inv_g); };
+  int lim;
+  {
+    const int64_t v = (int64_t)it.vis0 + query_of(min(row, R - 1)) - it.tok_begin;
+    lim = (int)std::min<int64_t>(it.tok_count, std::max<int64_t>(v, 0));
+  }
+  const int lim_most = __builtin_amdgcn_readlane(lim, 31);   // rows are in query order
+  const int unseen = (int)std::min<int64_t>(it.tok_count, std::max<int64_t>((int64_t)it.vis0 - it.tok_begin, 0));
+
+  // ---- Q as the B operand: lane holds Q[row][16 ks + 8 h .. +7]; a negative scale moves
+  // its sign into Q, a zero one zeroes Q (the softmax takes the max of unscaled scores)
+  v8s qf[KS];
+  if (row < R) {
+    const int j = query_of(row), hh = row - j * g;
+    const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(it.q_begin + j) * a.q_sn + (int64_t)(kvh * g + hh) * a.q_sh;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const v8s*>(qp + ks * 16 + h * 8);
+    if (a.scale_log2 <= 0.f) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[ks] = a.scale_log2 == 0.f ? (v8s)(short)0 : qf[ks] ^ (v8s)(short)0x8000;
+    }
+  } else {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
+  }
+  __syncthreads();                                   // page ids and scales staged
+  const int k_ref = max(k_top, 27);                  // (27: the least exponent; pages not written have byte 0)
+  const float scale = (a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2)) * __uint_as_float((uint32_t)k_ref << 23);
+
+  // ---- tile loads: thread's chunks tid + 256 i of K and of V
+  const int slot0 = it.tok_begin - first_page * ps;
+  const float inv_ps = 1.f / (float)ps;
+  const uint32_t row_bytes = (uint32_t)a.hkv * D;
+  const uint8_t* kv = reinterpret_cast<const uint8_t*>(a.kv) + (int64_t)kvh * D;
+  v4i kc[NC], vc[NC];
+  int sc[NC];
+  auto fetch = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = tid + 256 * i, t = tile * kTile + c / CPR;
+      kc[i] = vc[i] = v4i{0, 0, 0, 0};               // (past the end: scores are masked, V is zeros)
+      sc[i] = 0;
+      if (t < it.tok_count) {
+        const int pi = (int)(((float)(slot0 + t) + 0.5f) * inv_ps), sl = slot0 + t - pi * ps;
+        sc[i] = sc_lds[pi];
+        const uint8_t* src = kv + ((uint64_t)((uint32_t)pg_lds[pi] * 2u) * (uint32_t)ps + (uint32_t)sl) * row_bytes + (c % CPR) * 16;
+        kc[i] = *reinterpret_cast<const v4i*>(src);
+        vc[i] = *reinterpret_cast<const v4i*>(src + (uint64_t)ps * row_bytes);
+      }
+    }
+  };
+  auto put = [&](int tile, unsigned char* to) {
+    const bool masked = unseen < min(it.tok_count, (tile + 1) * kTile);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = tid + 256 * i, r = c / CPR, ch = (c % CPR) * 2;
+      if (masked && __builtin_expect((nan_bytes(vc[i][0]) | nan_bytes(vc[i][1]) | nan_bytes(vc[i][2]) | nan_bytes(vc[i][3])) != 0, 0)) {
+        // tokens that a row must not see: their NaN would reach it by a weight of 0
+#pragma unroll
+        for (int b = 0; b < 16; ++b)
+          if (((vc[i][b >> 2] >> (8 * (b & 3))) & 0x7f) == 0x7f) {
+            atomicMin(&nan_tok[(c % CPR) * 16 + b], tile * kTile + r);
+            vc[i][b >> 2] &= ~(0xff << (8 * (b & 3)));
+          }
+        nan_any = 1;
+      }
+      const float ks = __uint_as_float((uint32_t)max((sc[i] & 0xff) - k_ref + 127, 0) << 23), vs = __uint_as_float((uint32_t)(sc[i] >> 8) << 23);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t at = r * RB + (((ch + half) ^ swz16<D>(r)) << 4);
+        *reinterpret_cast<u4*>(to + at) = u4{value2<T, false>(kc[i][2 * half], ks), value2<T, true>(kc[i][2 * half], ks),
+                                             value2<T, false>(kc[i][2 * half + 1], ks), value2<T, true>(kc[i][2 * half + 1], ks)};
+        *reinterpret_cast<u4*>(to + PLANE + at) = u4{value2<T, false>(vc[i][2 * half], vs), value2<T, true>(vc[i][2 * half], vs),
+                                                     value2<T, false>(vc[i][2 * half + 1], vs), value2<T, true>(vc[i][2 * half + 1], vs)};
+      }
+    }
+  };
+
+  // ---- operand offsets
+  const int r16 = lane & 15, q4 = r16 >> 2, e4 = ((lane >> 4) & 1) * 2 + ((r16 & 3) >> 1);
+  uint32_t koff[KS], voff[MB][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) koff[ks] = lr * RB + (((2 * ks + h) ^ swz16<D>(lr)) << 4);
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int vr = 8 * u + 4 * h + q4;             // the row's low four bits
+      voff[mb][u] = vr * RB + (((mb * 4 + e4) ^ swz16<D>(vr)) << 4) + (r16 & 1) * 8;
+    }
+
+  // reference of the sums, the largest score (both times `scale`), the weights' sum
+  float m_run = -INFINITY, m_top = -INFINITY, l_run = 0.f;
+  v16f o_acc[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o_acc[mb][i] = 0.f;
+
+  fetch(0);
+  put(0, stage);
+  if (n_tiles > 1) fetch(1);
+  for (int tile = 0; tile < n_tiles; ++tile) {
+    const int st = tile & 1;
+    stream::lds_sync();                              // the tile is in its stage, and everyone is done with the other
+    if (tile + 1 < n_tiles) {
+      put(tile + 1, stage + (st ^ 1) * STAGE);
+      if (tile + 2 < n_tiles) fetch(tile + 2);
+    }
+    const int t0 = tile * kTile;
+    if (!wave_on || t0 >= lim_most) continue;
+    const unsigned char* kt = stage + st * STAGE;
+    const unsigned char* vt = kt + PLANE;
+
+    v16f x[2];
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[tb][i] = 0.f;
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb) {
+      v8s kf[KS];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const v8s*>(kt + tb * 32 * RB + koff[ks]);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) x[tb] = mfma32<T>(kf[ks], qf[ks], x[tb]);
+    }
+    if (__builtin_amdgcn_ballot_w64(lim < t0 + kTile) != 0) {
+      const int left = lim - t0 - 4 * h;
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (tb * 32 + 8 * (i >> 2) + (i & 3) >= left) x[tb][i] = -INFINITY;
+    }
+    // (maximum rather than fmax: a NaN score makes the row NaN either way)
+    float top = -INFINITY;
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2)
+        top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(x[tb][i], x[tb][i + 1]), top);
+    // When a row's largest score grows, every row of the wave takes the tile's largest as
+    // its reference, unless it lies 2^8 below the row's: that weight is exact in 16 bits
+    top = other_half(top, false) * scale;
+    if (__builtin_amdgcn_ballot_w64(top > m_top) != 0) {
+      m_top = fmaxf(m_top, top);
+      const float m_new = top >= m_top - 8.f ? top : m_run;
+      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
+      l_run *= alpha;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) o_acc[mb] *= alpha;
+      m_run = m_new;
+    }
+    const float msafe = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      v4s vf[MB][2];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          vf[mb][u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((stream::lds_v4s_t)(vt + s * 16 * RB + voff[mb][u]));
+      uint32_t pw[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(x[s >> 1][8 * (s & 1) + 2 * j], scale, -msafe));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(x[s >> 1][8 * (s & 1) + 2 * j + 1], scale, -msafe));
+        l_run += p0 + p1;
+        pw[j] = stream::pack2<T>(p0, p1);
+      }
+      const v8s pf = __builtin_bit_cast(v8s, (u4){pw[0], pw[1], pw[2], pw[3]});
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+        o_acc[mb] = mfma32<T>(__builtin_shufflevector(vf[mb][0], vf[mb][1], 0, 1, 2, 3, 4, 5, 6, 7), pf, o_acc[mb]);
+    }
+  }
+
+  // ---- writes: lane holds Oᵀ[32 mb + 8 (i / 4) + 4 h + i % 4][row]
+  l_run = other_half(l_run, true);
+  const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+  const int j = query_of(row), hh = row - j * g, head = kvh * g + hh;
+  __syncthreads();                                   // every wave is done with the stages
+  if (nan_any) {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (nan_tok[32 * mb + 8 * (i >> 2) + 4 * h + (i & 3)] < lim) o_acc[mb][i] = NAN;
+  }
+  if (it.out_row < 0) {
+    // through LDS (the wave's own 32 rows, chunks swizzled by row), so that the stores
+    // are whole rows, 16 bytes a lane
+    unsigned char* ol = stage + w * kWaveRows * RB;
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const u2 pk = {stream::pack2<T>(o_acc[mb][4 * b] * inv, o_acc[mb][4 * b + 1] * inv),
+                       stream::pack2<T>(o_acc[mb][4 * b + 2] * inv, o_acc[mb][4 * b + 3] * inv)};
+        *reinterpret_cast<u2*>(ol + lr * RB + (((mb * 4 + b) ^ swz16<D>(lr)) << 4) + 8 * h) = pk;
+      }
+    // (a wave reads only what it wrote: the compiler's lgkmcnt waits order it)
+#pragma unroll
+    for (int i = 0; i < kWaveRows / RPI; ++i) {
+      const int lrow = i * RPI + lane / CPR16, orow = w * kWaveRows + lrow;
+      const uint4 v = *reinterpret_cast<const uint4*>(ol + lrow * RB + (((lane % CPR16) ^ swz16<D>(lrow)) << 4));
+      if (orow < R) {
+        const int oj = query_of(orow), oh = kvh * g + (orow - oj * g);
+        T* op = reinterpret_cast<T*>(a.out) + (int64_t)(it.q_begin + oj) * a.o_sn + (int64_t)oh * a.o_sh;
+        *reinterpret_cast<uint4*>(op + (lane % CPR16) * 8) = v;
+      }
+    }
+  } else if (row < R) {
+    float* op = a.part_o + ((int64_t)(it.out_row + j) * a.hq + head) * D;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const v4f v = {o_acc[mb][4 * b] * inv, o_acc[mb][4 * b + 1] * inv, o_acc[mb][4 * b + 2] * inv,
+                       o_acc[mb][4 * b + 3] * inv};
+        *reinterpret_cast<v4f*>(op + mb * 32 + 8 * b + 4 * h) = v;
+      }
+  }
+  if (row < R && h == 0) store_lse(a, it, j, head, m_run, l_run);
+}
+
+template <typename T, int D>
+static int launch_block(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st) {
+  const int n = info->num_wg;
+  if (n == 0) return BE_OK;
+  attn_kv8_block_kernel<T, D><<<(unsigned)n * (unsigned)info->num_kv_heads, 256, 0, st>>>(a, n);
   BE_HIP_CHECK(hipGetLastError());
   return BE_OK;
 }
 
 template <typename T>
 static int launch_d(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st) {
+  if (info->num_wg < 0 || info->num_wg > info->grid_items || (info->num_wg > 0 && info->head_dim == 256))
+    return fail(BE_ERR_INVALID, "corrupt plan: %d block items of %d at head_dim %d", info->num_wg, info->grid_items, info->head_dim);
   switch (info->head_dim) {
-    case 64: return launch_tile<T, 64>(info, a, st);
-    case 128: return launch_tile<T, 128>(info, a, st);
+    case 64:
+      if (const int rc = launch_block<T, 64>(info, a, st)) return rc;
+      return launch_tile<T, 64>(info, a, st);
+    case 128:
+      if (const int rc = launch_block<T, 128>(info, a, st)) return rc;
+      return launch_tile<T, 128>(info, a, st);
     case 256: return launch_tile<T, 256>(info, a, st);
     default: return fail(BE_ERR_UNSUPPORTED, "head_dim %d", info->head_dim);
   }

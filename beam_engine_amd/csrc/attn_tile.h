@@ -262,7 +262,8 @@ int f32_launch(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st)
 // per (item, KV head).
 int kv8_launch(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st);
 constexpr int kMaxPageKv8 = 1024;      // tokens of a page of an 8-bit cache
-constexpr int kMaxRowsKv8 = 64;        // rows of its items
+// Rows of its items: above 64 the block kernel's.
+inline int kv8_max_rows(int head_dim) { return head_dim == 256 ? 64 : kMaxTileRows; }
 
 // ---------------------------------------------------------------- 128-row blocks (attn_block.hip)
 // A streaming plan's stream_loop when its causal groups run as 128-row blocks.
