@@ -486,7 +486,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   int64_t chunk = ceil_div(work * hkv, target);
   chunk = std::max<int64_t>(128, ceil_div(chunk, 64) * 64);
   // an item's page ids are staged in LDS: at most kMaxPagesLds pages per item
-  const int64_t chunk_cap = std::max<int64_t>(64, ((int64_t)(kMaxPagesLds - 1) * page_size) / 64 * 64);
+  const int64_t chunk_cap = std::max<int64_t>(64, ((int64_t)((kv8 ? kMaxPagesKv8 : kMaxPagesLds) - 1) * page_size) / 64 * 64);
   if (chunk > chunk_cap) chunk = chunk_cap;
 
   // A chunk of a group writes rows x D x 4 bytes of partials per KV head while
@@ -531,7 +531,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
         // clamping to [0, kv_len]: may be negative), query j of the item sees
         // vis0 + j (the kernel clamps per row); kNoCausal without the mask
         const int vis0 = gr.kv_len - (gr.q1 - gr.q0) + (qa - gr.q0) + 1;
-        WorkItem w{qa, qn, gr.page_base, t0, tc, -1, is_causal(gr) ? vis0 : kNoCausal, 0};
+        WorkItem w{qa, qn, gr.page_base, t0, tc, -1, is_causal(gr) ? vis0 : kNoCausal, kv8 ? t0 / page_size : 0};
         if (!direct) {
           w.out_row = rows;
           for (int j = 0; j < qn; ++j) rows_of[qa + j].push_back(rows + j);

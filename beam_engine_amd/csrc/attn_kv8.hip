@@ -4,7 +4,7 @@
 //
 // One workgroup of four waves per (work item, KV head): RT 16-row tiles of the item's
 // rows (queries x GQA group) over its tokens in 64-token tiles.  Codes go global -> LDS
-// directly, two tiles in flight; a wave reads its MFMA operands from LDS as codes and
+// directly, two tiles ahead; a wave reads its MFMA operands from LDS as codes and
 // turns them into 16-bit values in registers (v_cvt_scalef32_pk), so neither HBM nor
 // LDS moves a 16-bit K or V.  K's scale multiplies the fp32 scores, V's the conversion:
 // both exact (fp16 values of V below 2^-14 round to its subnormal step of 2^-24).
@@ -68,14 +68,14 @@ __device__ __forceinline__ int swz(int r) {
 // Takes NaN codes out of a V tile in LDS, noting the first such token of each column:
 // the rows that see it get their NaN at the end.  (By all threads of the workgroup, on
 // tiles with tokens that some row must not see.)
-template <int D>
+template <int D, int (*SWZ)(int)>
 __device__ __forceinline__ void set_nans_aside(unsigned char* v, int tok0, int tid, int32_t* nan_tok, int32_t* nan_any) {
   constexpr int CPR = D / 16;
 #pragma unroll 1
   for (int c = tid; c < kTile * CPR; c += 256) {
     const v4i w = *reinterpret_cast<const v4i*>(v + c * 16);
     if (__builtin_expect((nan_bytes(w[0]) | nan_bytes(w[1]) | nan_bytes(w[2]) | nan_bytes(w[3])) == 0, 1)) continue;
-    const int row = c / CPR, col = ((c % CPR) ^ swz<CPR>(row)) * 16;
+    const int row = c / CPR, col = ((c % CPR) ^ SWZ(row)) * 16;
 #pragma unroll 1
     for (int b = 0; b < 16; ++b)
       if ((v[c * 16 + b] & 0x7f) == 0x7f) {
@@ -95,50 +95,174 @@ __device__ __forceinline__ void store_lse(const AttnArgs& a, const WorkItem& it,
 
 // What a workgroup keeps in LDS.
 template <int D> struct TileShared {
-  unsigned char stage[2 * 2 * kTile * D];
-  int32_t pg[kMaxPagesLds];
-  uint16_t sc[kMaxPagesLds];           // scale bytes of the pages: K | V << 8
+  static constexpr int kStages = D == 256 ? 2 : 3;   // tiles in LDS
+  unsigned char stage[kStages * 2 * kTile * D];
+  int32_t pg[kMaxPagesKv8];
+  uint32_t ks[kMaxPagesKv8], vs[kMaxPagesKv8];       // scale bytes of the pages
   int32_t nan_tok[D];                  // per column: the first masked tile's token whose V is NaN
   int32_t nan_any;
 };
+static_assert(kMaxPagesKv8 == 256, "a thread stages one page");
 
-template <typename T, int D, int RT, bool PAGED4, bool QUADS>
+// One byte a lane, global -> LDS dwords lds + 4 lane (zero-extended), as stream::dma16.
+__device__ __forceinline__ void dma_byte(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
+}
+
+// An item's pages: ids and scale bytes to LDS, and the K and V codes of its tiles,
+// global -> LDS directly.  The chain of a workgroup's start is three round trips: the
+// item's record, page ids (with Q), scales and the first tiles.  The scales leave ahead
+// of the tiles, so a wait for the first tile is one for them.
+//
+// PAGED: pages hold whole loads' rows (1 KB), so a load's page is wave-uniform: its id
+// comes from a register (64 of the item's ids) by v_readlane and its address is scalar.
+// Otherwise every lane looks its row's page up in LDS.  Past the item's end K re-reads
+// its last token (the scores are masked) and V reads zeros.
+template <int D, bool PAGED, int (*SWZ)(int)>
+struct Codes {
+  static constexpr int CPR = D / 16, RPI = 64 / CPR;   // 16-byte chunks per row, rows per wave load
+  static constexpr int IPW = kTile / RPI / 4;          // loads per wave per tile (K and V each)
+  static constexpr int PLANE = kTile * D, STAGE = 2 * PLANE;
+
+  uint64_t kvb;
+  uint32_t row_bytes, page_bytes, vplane, off;
+  int w, lane, ps, tok_count, slot0, n_pages, tok;
+  float inv_ps;
+  int page[IPW], slot[IPW], dpage, dslot;              // PAGED: of the next tile's loads
+  int id, pg_reg, pg_base;
+  const int32_t* pg_lds;
+
+  // Page of the item's token t: pages hold at most 1024 tokens and an item 256 pages.
+  __device__ __forceinline__ int page_of(int t) const {
+    return min((int)(((float)(slot0 + t) + 0.5f) * inv_ps), n_pages - 1);
+  }
+
+  // The page ids leave; nothing waits for them yet.
+  __device__ __forceinline__ void begin(const AttnArgs& a, const WorkItem& it, int kvh, int wave) {
+    w = wave;
+    lane = threadIdx.x & 63;
+    ps = a.page_size;
+    inv_ps = 1.f / (float)ps;
+    tok_count = it.tok_count;
+    slot0 = it.tok_begin - it.first_page * ps;
+    n_pages = (int)(((float)(slot0 + tok_count - 1) + 0.5f) * inv_ps) + 1;
+    const int32_t* pages = a.pages + it.page_begin + it.first_page;
+    id = pages[min((int)threadIdx.x, n_pages - 1)];
+    pg_reg = PAGED ? pages[min(lane, n_pages - 1)] : 0;
+    row_bytes = (uint32_t)a.hkv * D;
+    vplane = (uint32_t)ps * row_bytes;
+    page_bytes = 2 * vplane;
+    kvb = reinterpret_cast<uint64_t>(a.kv) + (uint64_t)kvh * D;
+    tok = 0;
+    pg_base = 0;
+    // (the swizzle of a load's rows: r0 + lane / CPR differs from lane / CPR by a multiple of RPI)
+    off = (uint32_t)(lane / CPR) * row_bytes;
+    if constexpr (PAGED) {
+      dpage = (int)(((float)kTile + 0.5f) * inv_ps);
+      dslot = kTile - dpage * ps;
+#pragma unroll
+      for (int i = 0; i < IPW; ++i) {
+        const int t = slot0 + (w * IPW + i) * RPI;
+        page[i] = (int)(((float)t + 0.5f) * inv_ps);
+        slot[i] = t - page[i] * ps;
+      }
+    }
+  }
+
+  // Ids to LDS, scales on their way there.
+  __device__ __forceinline__ void stage(const AttnArgs& a, int kvh, int32_t* pg, uint32_t* ks, uint32_t* vs) {
+    pg[threadIdx.x] = id;
+    pg_lds = pg;
+    const uint8_t* sc = a.kv_scale + (int64_t)id * 2 * a.hkv + kvh;
+    dma_byte(sc, lds_addr(ks) + w * 256);
+    dma_byte(sc + a.hkv, lds_addr(vs) + w * 256);
+    if constexpr (!PAGED) __syncthreads();
+  }
+
+  template <bool WHOLE>
+  __device__ __forceinline__ void rows(uint32_t dst0) {
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) {
+      const int r0 = (w * IPW + i) * RPI, lr = lane / CPR;
+      const uint32_t dst = dst0 + (w * IPW + i) * 1024, ch = (uint32_t)((lane % CPR) ^ SWZ(r0 + lr)) << 4;
+      const int left = tok_count - 1 - (tok + r0);     // rows of this load up to the item's last token
+      if constexpr (PAGED) {
+        int pg = page[i], sl = slot[i];
+        if (!WHOLE && left < 0) {                      // the load lies past the end: the last token's row
+          pg = n_pages - 1;
+          sl = slot0 + tok_count - 1 - pg * ps;
+        }
+        const uint32_t pid = (uint32_t)__builtin_amdgcn_readlane(pg_reg, pg - pg_base);
+        const uint64_t base = kvb + (uint64_t)pid * page_bytes + (uint32_t)sl * row_bytes;
+        const uint32_t o = (WHOLE ? off : (uint32_t)min(lr, max(left, 0)) * row_bytes) + ch;
+        stream::dma16_sv(base, o, dst);
+        if constexpr (WHOLE) {
+          stream::dma16_sv(base + vplane, o, dst + PLANE);
+        } else {
+          stream::dma16(lr <= left ? reinterpret_cast<const void*>(base + vplane + o) : &kZeroChunk, dst + PLANE);
+        }
+        slot[i] += dslot;
+        const bool carry = slot[i] >= ps;
+        slot[i] -= carry ? ps : 0;
+        page[i] += dpage + (carry ? 1 : 0);
+      } else {
+        const bool in = WHOLE || lr <= left;
+        const int t = in ? tok + r0 + lr : tok_count - 1, pg = page_of(t), sl = slot0 + t - pg * ps;
+        const uint64_t src = kvb + (uint64_t)(uint32_t)pg_lds[pg] * page_bytes + (uint32_t)sl * row_bytes + ch;
+        stream::dma16(reinterpret_cast<const void*>(src), dst);
+        stream::dma16(in ? reinterpret_cast<const void*>(src + vplane) : &kZeroChunk, dst + PLANE);
+      }
+    }
+  }
+
+  // The next tile's loads, to LDS byte address dst0 (2 IPW vector memory operations).
+  __device__ __forceinline__ void load(uint32_t dst0) {
+    if constexpr (PAGED) {
+      // (a tile's pages lie within 64 of its first; pg_lds is read from the third tile on,
+      // behind a barrier: the first two lie within the register's first 64 pages)
+      if (min(page[IPW - 1], n_pages - 1) - pg_base >= 64) {
+        pg_base = min(page[0], n_pages - 1);
+        pg_reg = pg_lds[min(pg_base + lane, n_pages - 1)];
+      }
+    }
+    if (__builtin_expect(tok + kTile <= tok_count, 1)) rows<true>(dst0);
+    else rows<false>(dst0);
+    tok += kTile;
+  }
+
+  // Waits until the tile that was loaded `newer` loads ago is whole, for everyone.
+  template <int newer> static __device__ __forceinline__ void wait() {
+    constexpr int N = 2 * IPW * newer;
+    if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else if constexpr (N == 2) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+};
+
+template <typename T, int D, int RT, bool PAGED, bool QUADS>
 __device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& it, TileShared<D>& sh) {
   constexpr int CPR = D / 16;                        // 16-code chunks of a row
-  using Loader = TileLoader<D, PAGED4, swz<CPR>>;
-  constexpr int PLANE = Loader::PLANE, STAGE = Loader::STAGE;
+  using Loader = Codes<D, PAGED, swz<CPR>>;
+  constexpr int PLANE = Loader::PLANE, STAGE = Loader::STAGE, NST = TileShared<D>::kStages;
   constexpr int KP = D / 64;                         // K chunk quads: two QK contraction steps each
   constexpr int TS = RT == 4 ? 1 : 2;                // waves sharing a row tile: token halves,
   constexpr int CS = RT == 1 ? 2 : 1;                // and head_dim halves of Oᵀ
   constexpr int NSUB = 4 / TS;                       // 16-token sub-tiles per wave per tile
   constexpr int MT = D / 16 / CS;                    // Oᵀ head_dim tiles of a wave
   constexpr int COMB_SLOT = (MT * 64 * 4 + 2 * 64) * 4;
-  static_assert(TS == 1 || 2 * COMB_SLOT <= 2 * STAGE, "combine scratch must fit");
+  static_assert(TS == 1 || 2 * COMB_SLOT <= TileShared<D>::kStages * STAGE, "combine scratch must fit");
 
   unsigned char* stage = sh.stage;
-  int32_t* pg_lds = sh.pg;
-  uint16_t* sc_lds = sh.sc;
   int32_t* nan_tok = sh.nan_tok;
   const int kvh = blockIdx.y;
   const int tid = threadIdx.x;
   const int w = rfl(tid >> 6), lane = tid & 63, lg = lane >> 4, lc = lane & 15;
-  const int g = a.g, R = it.q_count * g, ps = a.page_size;
-
-  // ---- the item's pages
-  const int first_page = it.tok_begin / ps;
-  const int n_pages = (it.tok_begin + it.tok_count - 1) / ps - first_page + 1;
+  const int g = a.g, R = it.q_count * g;
   const int n_tiles = (it.tok_count + kTile - 1) / kTile;
   const uint32_t lds0 = lds_addr(stage);
   Loader ld;
-  if constexpr (PAGED4) {
-    ld.init(a, it, kvh, w, pg_lds, first_page, n_pages);
-    for (int i = 64 + tid; i < n_pages; i += 256) pg_lds[i] = a.pages[it.page_begin + first_page + i];
-    if (tid < min(n_pages, 64)) pg_lds[tid] = ld.pg_reg;
-  } else {
-    for (int i = tid; i < n_pages; i += 256) pg_lds[i] = a.pages[it.page_begin + first_page + i];
-    __syncthreads();
-    ld.init(a, it, kvh, w, pg_lds, first_page, n_pages);
-  }
+  ld.begin(a, it, kvh, w);
 
   // ---- wave role
   const int rt = RT == 1 ? 0 : w % RT, ts = RT == 4 ? 0 : RT == 2 ? w >> 1 : w & 1, cs = RT == 1 ? w >> 1 : 0;
@@ -157,23 +281,18 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& it,
 #pragma unroll
     for (int x = 0; x < 2 * KP; ++x) qf[x] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
   }
+  // Q, which left with the page ids, has landed before the tile loads go out: a later
+  // first use would make the compiler wait for them too
 #pragma unroll
   for (int x = 0; x < 2 * KP; ++x) asm volatile("" : "+v"(qf[x]));
-  ld.load(lds0);
-  if (n_tiles > 1) ld.load(lds0 + STAGE);
+  ld.stage(a, kvh, sh.pg, sh.ks, sh.vs);
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i)
+    if (i < n_tiles) ld.load(lds0 + i * STAGE);
   for (int i = tid; i < D; i += 256) nan_tok[i] = INT32_MAX;
   if (tid == 0) sh.nan_any = 0;
-  // ---- the pages' scales (behind the first tiles' loads, which they need not precede)
-  for (int i = tid; i < n_pages; i += 256) {
-    const int64_t at = (int64_t)a.pages[it.page_begin + first_page + i] * 2 * a.hkv + kvh;
-    sc_lds[i] = (uint16_t)(a.kv_scale[at] | (uint32_t)a.kv_scale[at + a.hkv] << 8);
-  }
-  // page of the item's token t: pages hold at most 1024 tokens and an item 1024 pages
-  const int slot0 = it.tok_begin - first_page * ps;
-  const float inv_ps = 1.f / (float)ps;
-  auto page_of = [&](int t) { return min((int)(((float)(slot0 + t) + 0.5f) * inv_ps), n_pages - 1); };
-  auto k_scale = [&](int t) { return __uint_as_float((uint32_t)(sc_lds[page_of(t)] & 0xff) << 23); };
-  auto v_scale = [&](int t) { return __uint_as_float((uint32_t)(sc_lds[page_of(t)] >> 8) << 23); };
+  auto k_scale = [&](int t) { return __uint_as_float(sh.ks[ld.page_of(t)] << 23); };
+  auto v_scale = [&](int t) { return __uint_as_float(sh.vs[ld.page_of(t)] << 23); };
   // item tokens this lane's row sees (causal: its query's limit)
   int lim;
   {
@@ -197,20 +316,17 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& it,
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) o_acc[mt] = v4f{0.f, 0.f, 0.f, 0.f};
 
-  for (int tile = 0; tile < n_tiles; ++tile) {
-    const int st = tile & 1;
-    // this wave's loads of the tile have landed (the next tile's may be in
-    // flight); after the barrier everyone's have
-    if (tile + 1 < n_tiles) {
-      if constexpr (Loader::IPW == 1) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      else if constexpr (Loader::IPW == 2) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    }
+  int st = 0;
+  for (int tile = 0; tile < n_tiles; ++tile, st = st + 1 == NST ? 0 : st + 1) {
+    // this wave's loads of the tile have landed (those of the next NST - 2 may be in
+    // flight); after the barrier everyone's have, and everyone is done with the tile
+    // before, whose stage the tile NST - 1 ahead takes
+    if (NST > 2 && tile + 1 < n_tiles) Loader::template wait<1>();
+    else Loader::template wait<0>();
+    if (tile + NST - 1 < n_tiles) ld.load(lds0 + (st == 0 ? NST - 1 : st - 1) * STAGE);
     if (unseen < min(it.tok_count, (tile + 1) * kTile)) {
       // tokens that a row must not see: their NaN would reach it by a weight of 0
-      set_nans_aside<D>(stage + st * STAGE + PLANE, tile * kTile, tid, nan_tok, &sh.nan_any);
+      set_nans_aside<D, swz<CPR>>(stage + st * STAGE + PLANE, tile * kTile, tid, nan_tok, &sh.nan_any);
       stream::lds_sync();
     }
     const int s0 = tile * kTile + ts * NSUB * 16;      // first token of the wave's sub-tiles
@@ -297,11 +413,6 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& it,
         }
       }
     }
-    if (tile + 2 < n_tiles) {
-      // everyone is done with this stage
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      ld.load(lds0 + st * STAGE);
-    }
   }
   l_run = rows4_sum(l_run);
 
@@ -358,18 +469,286 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& it,
   }
 }
 
+constexpr int kWaveRows = 32;
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+template <typename T> __device__ __forceinline__ v16f mfma32(v8s a, v8s b, v16f c) {
+  if constexpr (std::is_same<T, bf16_t>::value) {
+    typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+  } else {
+    typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+  }
+}
+
+// The value of the lane with the other bit 5 (the other token quads of the same row).
+__device__ __forceinline__ float other_half(float x, bool sum) {
+  typedef unsigned int u2 __attribute__((ext_vector_type(2)));
+  const unsigned xb = __float_as_uint(x);
+  const u2 r = __builtin_amdgcn_permlane32_swap(xb, xb, false, false);
+  const unsigned a = r.x, b = r.y;
+  return sum ? __uint_as_float(a) + __uint_as_float(b) : fmaxf(__uint_as_float(a), __uint_as_float(b));
+}
+
+// ================================================================== 32-row tiles
+// The same of the 32-row tiles below: 16 consecutive rows' chunk, and the rows 4 h .. + 3
+// and 8 + 4 h .. + 3 by two chunks of a half wave's transposed V read.
+template <int CPR>
+__device__ __forceinline__ int swz32(int r) {
+  return CPR == 8 ? ((r >> 1) & 1) << 1 | ((r >> 3) & 1) << 2 | ((r >> 2) & 1) : ((r >> 3) & 1) << 1 | ((r >> 2) & 1);
+}
+
+// Items of 17 to 64 rows (a prefix that some beams share), head_dim 64 or 128: RT 32-row
+// tiles on v_mfma_f32_32x32x16, so that an operand's conversion serves 32 rows; two
+// waves share a row tile's tokens (and with one row tile two its columns).  The C layout
+// of a 32-token Sᵀ block (lane l: row l % 32, tokens 8 (i / 4) + 4 (l / 32) + i % 4) is,
+// eight registers at a time, the B operand of Oᵀ += Vᵀ Pᵀ over the token order that the
+// transposed V reads follow.
+template <typename T, int D, int RT, bool PAGED, bool QUADS>
+__device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& it, TileShared<D>& sh) {
+  constexpr int CPR = D / 16;                        // 16-code chunks of a row
+  using Loader = Codes<D, PAGED, swz32<CPR>>;
+  constexpr int PLANE = Loader::PLANE, STAGE = Loader::STAGE, NST = TileShared<D>::kStages;
+  constexpr int KP = D / 32;                         // K chunk pairs: two QK contraction steps each
+  constexpr int CS = RT == 1 ? 2 : 1;
+  constexpr int MB = D / 32 / CS;                    // Oᵀ head_dim blocks of a wave
+  constexpr int COMB_SLOT = (MB * 16 * 64 + 2 * 64) * 4;
+  static_assert(2 * COMB_SLOT <= NST * STAGE && RT * 32 * D * 4 <= NST * STAGE, "scratch must fit");
+
+  unsigned char* stage = sh.stage;
+  const int kvh = blockIdx.y;
+  const int tid = threadIdx.x;
+  const int w = rfl(tid >> 6), lane = tid & 63, h = lane >> 5, lr = lane & 31;
+  const int g = a.g, R = it.q_count * g;
+  const int n_tiles = (it.tok_count + kTile - 1) / kTile;
+  const uint32_t lds0 = lds_addr(stage);
+  Loader ld;
+  ld.begin(a, it, kvh, w);
+
+  // ---- wave role
+  const int rt = RT == 1 ? 0 : w & 1, ts = RT == 1 ? w & 1 : w >> 1, cs = RT == 1 ? w >> 1 : 0;
+  const bool active = rt * 32 < R;
+  const int row = rt * 32 + lr;
+  // row / g for row < 256 (the quotient's distance from an integer is at least 1 / (2 g))
+  const int j = (int)(((float)row + 0.5f) * (1.f / (float)g)), hh = row - j * g;
+
+  // ---- Q as the B operand: product 2 kp + i takes head_dim 16 (2 kp + h) + 8 i .. + 7
+  v8s qf[2 * KP];
+  if (row < R) {
+    const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(it.q_begin + j) * a.q_sn + (int64_t)(kvh * g + hh) * a.q_sh;
+#pragma unroll
+    for (int x = 0; x < 2 * KP; ++x) qf[x] = *reinterpret_cast<const v8s*>(qp + 16 * (2 * (x >> 1) + h) + 8 * (x & 1));
+  } else {
+#pragma unroll
+    for (int x = 0; x < 2 * KP; ++x) qf[x] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int x = 0; x < 2 * KP; ++x) asm volatile("" : "+v"(qf[x]));
+  ld.stage(a, kvh, sh.pg, sh.ks, sh.vs);
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i)
+    if (i < n_tiles) ld.load(lds0 + i * STAGE);
+  for (int i = tid; i < D; i += 256) sh.nan_tok[i] = INT32_MAX;
+  if (tid == 0) sh.nan_any = 0;
+  int lim;
+  {
+    const int64_t v = (int64_t)it.vis0 + j - it.tok_begin;
+    lim = (int)std::min<int64_t>(it.tok_count, std::max<int64_t>(v, 0));
+  }
+  const int unseen = (int)std::min<int64_t>(it.tok_count, std::max<int64_t>((int64_t)it.vis0 - it.tok_begin, 0));
+  // ---- operand offsets (the swizzle repeats every 16 rows)
+  uint32_t koff[KP], voff[MB];
+#pragma unroll
+  for (int kp = 0; kp < KP; ++kp) koff[kp] = lr * D + (((2 * kp + h) ^ swz32<CPR>(lr)) << 4);
+  const int vj = (lane & 15) >> 1, vr = (vj >> 2) * 8 + 4 * h + (vj & 3);
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+    voff[mb] = vr * D + (((2 * (cs * MB + mb) + ((lane >> 4) & 1)) ^ swz32<CPR>(vr)) << 4) + (lane & 1) * 8;
+
+  float m_run = -INFINITY, l_run = 0.f;
+  v16f o_acc[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o_acc[mb][i] = 0.f;
+
+  int st = 0;
+  for (int tile = 0; tile < n_tiles; ++tile, st = st + 1 == NST ? 0 : st + 1) {
+    // (as in the 16-row tiles: this tile has landed, the tile before is done with)
+    if (NST > 2 && tile + 1 < n_tiles) Loader::template wait<1>();
+    else Loader::template wait<0>();
+    if (tile + NST - 1 < n_tiles) ld.load(lds0 + (st == 0 ? NST - 1 : st - 1) * STAGE);
+    if (unseen < min(it.tok_count, (tile + 1) * kTile)) {
+      set_nans_aside<D, swz32<CPR>>(stage + st * STAGE + PLANE, tile * kTile, tid, sh.nan_tok, &sh.nan_any);
+      stream::lds_sync();
+    }
+    const int s0 = tile * kTile + ts * 32;           // first token of the wave's block
+    if (!active || s0 >= it.tok_count) continue;
+    const unsigned char* kt = stage + st * STAGE + ts * 32 * D;
+    const unsigned char* vt = kt + PLANE;
+    // scales of the lane's tokens, quad 8 q + 4 h .. + 3 or one each
+    constexpr int NS = QUADS ? 4 : 16;
+    float ks[NS], vs[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int pg = ld.page_of(s0 + (QUADS ? 8 * i + 4 * h : 8 * (i >> 2) + 4 * h + (i & 3)));
+      ks[i] = __uint_as_float(sh.ks[pg] << 23) * a.scale_log2;
+      vs[i] = __uint_as_float(sh.vs[pg] << 23);
+    }
+    v16f x;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    v4i kc[KP];
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) kc[kp] = *reinterpret_cast<const v4i*>(kt + koff[kp]);
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+      x = mfma32<T>(codes8<T>(kc[kp][0], kc[kp][1]), qf[2 * kp], x);
+      x = mfma32<T>(codes8<T>(kc[kp][2], kc[kp][3]), qf[2 * kp + 1], x);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] *= ks[QUADS ? i >> 2 : i];
+    if (__builtin_amdgcn_ballot_w64(lim < s0 + 32) != 0) {
+      const int left = lim - s0 - 4 * h;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i >> 2) + (i & 3) >= left) x[i] = -INFINITY;
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+    mx = other_half(mx, false);
+    const float m_new = fmaxf(m_run, mx);
+    const float msafe = m_new == -INFINITY ? 0.f : m_new;
+    if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0) {
+      const float alpha = __builtin_amdgcn_exp2f(m_run - msafe);      // 0 while nothing was seen
+      l_run *= alpha;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) o_acc[mb] *= alpha;
+    }
+    m_run = m_new;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      uint32_t pw[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f(x[8 * s + 2 * i] - msafe), p1 = __builtin_amdgcn_exp2f(x[8 * s + 2 * i + 1] - msafe);
+        l_run += p0 + p1;
+        pw[i] = stream::pack2<T>(p0, p1);
+      }
+      const v8s pf = __builtin_bit_cast(v8s, (u4){pw[0], pw[1], pw[2], pw[3]});
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        const v2i vc = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i_t)(vt + s * 16 * D + voff[mb]));
+        u4 vv;
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          if constexpr (QUADS) {
+            vv[2 * o] = value2<T, false>(vc[o], vs[2 * s + o]);
+            vv[2 * o + 1] = value2<T, true>(vc[o], vs[2 * s + o]);
+          } else {
+            vv[2 * o] = value11<T, false>(vc[o], vs[8 * s + 4 * o], vs[8 * s + 4 * o + 1]);
+            vv[2 * o + 1] = value11<T, true>(vc[o], vs[8 * s + 4 * o + 2], vs[8 * s + 4 * o + 3]);
+          }
+        }
+        o_acc[mb] = mfma32<T>(__builtin_bit_cast(v8s, vv), pf, o_acc[mb]);
+      }
+    }
+  }
+  l_run = other_half(l_run, true);
+
+  // ---- the second token half hands its state to the first
+  float* comb = reinterpret_cast<float*>(stage);
+  {
+    float* slot = comb + (RT == 1 ? cs : rt) * (COMB_SLOT / 4);
+    __syncthreads();                                   // tiles no longer needed
+    if (ts > 0 && active) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v4f v = {o_acc[mb][4 * i], o_acc[mb][4 * i + 1], o_acc[mb][4 * i + 2], o_acc[mb][4 * i + 3]};
+          *reinterpret_cast<v4f*>(slot + ((mb * 4 + i) * 64 + lane) * 4) = v;
+        }
+      slot[MB * 1024 + lane] = m_run;
+      slot[MB * 1024 + 64 + lane] = l_run;
+    }
+    __syncthreads();
+    if (ts == 0 && active) {
+      const float mb_ = slot[MB * 1024 + lane], lb = slot[MB * 1024 + 64 + lane];
+      const float M = fmaxf(m_run, mb_);
+      const float ca = (M == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(m_run - M);
+      const float cb = (M == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(mb_ - M);
+      l_run = l_run * ca + lb * cb;
+      m_run = M;
+      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v4f v = *reinterpret_cast<const v4f*>(slot + ((mb * 4 + i) * 64 + lane) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o_acc[mb][4 * i + e] = (o_acc[mb][4 * i + e] * ca + v[e] * cb) * inv;
+        }
+      if (sh.nan_any) {
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (sh.nan_tok[32 * (cs * MB + mb) + 8 * (i >> 2) + 4 * h + (i & 3)] < lim) o_acc[mb][i] = NAN;
+      }
+      if (h == 0 && cs == 0 && row < R) store_lse(a, it, j, kvh * g + hh, m_run, l_run);
+    }
+    __syncthreads();                                   // the states have been read
+  }
+
+  // ---- writes, through LDS so that they are whole rows: lane holds
+  // Oᵀ[32 (cs MB + mb) + 8 (i / 4) + 4 h + i % 4][row]; rows of D floats, 16-byte chunk c at c ^ (row & 15)
+  if (ts == 0 && active) {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const v4f v = {o_acc[mb][4 * i], o_acc[mb][4 * i + 1], o_acc[mb][4 * i + 2], o_acc[mb][4 * i + 3]};
+        *reinterpret_cast<v4f*>(comb + row * D + (((8 * (cs * MB + mb) + 2 * i + h) ^ (row & 15)) << 2)) = v;
+      }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int c0 = 0; c0 < RT * 32 * (D / 4); c0 += 256) {
+    const int r = (c0 + tid) / (D / 4), ch = tid % (D / 4);
+    if (r >= R) break;
+    const int rj = (int)(((float)r + 0.5f) * (1.f / (float)g)), head = kvh * g + r - rj * g;
+    const v4f v = *reinterpret_cast<const v4f*>(comb + r * D + ((ch ^ (r & 15)) << 2));
+    if (it.out_row < 0) {
+      T* op = reinterpret_cast<T*>(a.out) + (int64_t)(it.q_begin + rj) * a.o_sn + (int64_t)head * a.o_sh;
+      *reinterpret_cast<v4s*>(op + 4 * ch) = pack4<T>(v[0], v[1], v[2], v[3]);
+    } else {
+      *reinterpret_cast<v4f*>(a.part_o + ((int64_t)(it.out_row + rj) * a.hq + head) * D + 4 * ch) = v;
+    }
+  }
+}
+
 // A workgroup takes as many row tiles as its item has: with fewer, the waves share out
 // the tokens of a row tile (and the columns) rather than idle.
-template <typename T, int D, bool PAGED4, bool QUADS>
-__global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_kv8_kernel(AttnArgs a, int first_item) {
+template <typename T, int D, bool PAGED, bool QUADS>
+__global__ __launch_bounds__(256, D == 256 || !QUADS ? 2 : D == 128 ? 3 : 4) void attn_kv8_kernel(AttnArgs a, int first_item) {
   __shared__ __attribute__((aligned(1024))) TileShared<D> sh;
   const int item = first_item + (int)blockIdx.x;
   if (a.live_items && item >= *a.live_items) return;
   const WorkItem it = a.items[item];
   const int R = it.q_count * a.g;
-  if (R <= 16) tile_item<T, D, 1, PAGED4, QUADS>(a, it, sh);
-  else if (R <= 32) tile_item<T, D, 2, PAGED4, QUADS>(a, it, sh);
-  else tile_item<T, D, 4, PAGED4, QUADS>(a, it, sh);
+  if (R <= 16) {
+    tile_item<T, D, 1, PAGED, QUADS>(a, it, sh);
+  } else if constexpr (D == 256) {                   // (32-row tiles would not fit the registers)
+    if (R <= 32) tile_item<T, D, 2, PAGED, QUADS>(a, it, sh);
+    else tile_item<T, D, 4, PAGED, QUADS>(a, it, sh);
+  } else {
+    if (R <= 32) tile32_item<T, D, 1, PAGED, QUADS>(a, it, sh);
+    else tile32_item<T, D, 2, PAGED, QUADS>(a, it, sh);
+  }
 }
 
 template <typename T, int D>
@@ -385,34 +764,11 @@ static int launch_tile(const be_attn_plan_info* info, const AttnArgs& a, hipStre
 }
 
 // ================================================================== 128-row blocks
-constexpr int kWaveRows = 32;
-typedef float v16f __attribute__((ext_vector_type(16)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-
-template <typename T> __device__ __forceinline__ v16f mfma32(v8s a, v8s b, v16f c) {
-  if constexpr (std::is_same<T, bf16_t>::value) {
-    typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
-  } else {
-    typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-  }
-}
-
 // The 16-byte chunk XOR of a row of 16-bit values: any 16 consecutive rows' chunk and
 // the four rows x four chunks of a half wave's transposed V read fall on all banks.
 template <int D>
 __device__ __forceinline__ int swz16(int r) {
   return D == 128 ? ((r & 3) << 2 | ((r >> 2) & 3)) : (((r >> 1) & 1) << 2 | ((r >> 2) & 3));
-}
-
-// The value of the lane with the other bit 5 (the other token quads of the same row).
-__device__ __forceinline__ float other_half(float x, bool sum) {
-  typedef unsigned int u2 __attribute__((ext_vector_type(2)));
-  const unsigned xb = __float_as_uint(x);
-  const u2 r = __builtin_amdgcn_permlane32_swap(xb, xb, false, false);
-  const unsigned a = r.x, b = r.y;
-  return sum ? __uint_as_float(a) + __uint_as_float(b) : fmaxf(__uint_as_float(a), __uint_as_float(b));
 }
 
 // Items of 65 to 128 rows (prompts, prefixes that many beams share), head_dim 64 or 128:
@@ -432,8 +788,8 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_block_kernel(AttnArgs a, int 
   constexpr int CPR16 = D / 8, RPI = 64 / CPR16;     // of the 16-bit rows
 
   __shared__ __attribute__((aligned(1024))) unsigned char stage[2 * STAGE];
-  __shared__ int32_t pg_lds[kMaxPagesLds];
-  __shared__ uint16_t sc_lds[kMaxPagesLds];
+  __shared__ int32_t pg_lds[kMaxPagesKv8];
+  __shared__ uint16_t sc_lds[kMaxPagesKv8];          // scale bytes of the pages: K | V << 8
   __shared__ int32_t nan_tok[D];
   __shared__ int32_t nan_any, k_top;
   // consecutive workgroups are the KV heads of one item: an XCD keeps the same heads in its L2
@@ -446,8 +802,10 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_block_kernel(AttnArgs a, int 
   const int g = a.g, R = it.q_count * g, ps = a.page_size;
 
   // ---- the item's pages and their scales
-  const int first_page = it.tok_begin / ps;
-  const int n_pages = (it.tok_begin + it.tok_count - 1) / ps - first_page + 1;
+  const int first_page = it.first_page;
+  const float inv_ps = 1.f / (float)ps;
+  const int slot0 = it.tok_begin - first_page * ps;
+  const int n_pages = (int)(((float)(slot0 + it.tok_count - 1) + 0.5f) * inv_ps) + 1;
   const int n_tiles = (it.tok_count + kTile - 1) / kTile;
   if (tid == 0) {
     nan_any = 0;
@@ -503,8 +861,6 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_block_kernel(AttnArgs a, int 
   const float scale = (a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2)) * __uint_as_float((uint32_t)k_ref << 23);
 
   // ---- tile loads: thread's chunks tid + 256 i of K and of V
-  const int slot0 = it.tok_begin - first_page * ps;
-  const float inv_ps = 1.f / (float)ps;
   const uint32_t row_bytes = (uint32_t)a.hkv * D;
   const uint8_t* kv = reinterpret_cast<const uint8_t*>(a.kv) + (int64_t)kvh * D;
   v4i kc[NC], vc[NC];

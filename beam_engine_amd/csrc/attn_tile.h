@@ -25,7 +25,7 @@ struct WorkItem {
   int32_t tok_count;   // tokens covered, > 0
   int32_t out_row;     // first partial row, or -1: write the final output
   int32_t vis0;        // causal: group tokens its first query sees, unclamped (query j: vis0 + j); else kNoCausal
-  int32_t pad1;
+  int32_t first_page;  // 8-bit caches: tok_begin / page_size
 };
 constexpr int32_t kNoCausal = 0x3fffffff;
 static_assert(sizeof(WorkItem) == 32, "WorkItem is 8 int32 words");
@@ -262,6 +262,7 @@ int f32_launch(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st)
 // per (item, KV head).
 int kv8_launch(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st);
 constexpr int kMaxPageKv8 = 1024;      // tokens of a page of an 8-bit cache
+constexpr int kMaxPagesKv8 = 256;      // pages of an item
 // Rows of its items: above 64 the block kernel's.
 inline int kv8_max_rows(int head_dim) { return head_dim == 256 ? 64 : kMaxTileRows; }
 

@@ -88,11 +88,12 @@ def test_plan_covers_every_token(hq, hkv, d, page):
     items = buf[info.off_items:info.off_items + 8 * info.num_items].reshape(-1, 8)
     for i, n in enumerate(lens):
         mine = sorted((int(x[3]), int(x[4])) for x in items if x[0] == i)
+        assert all(x[7] == x[3] // page for x in items)
         at = 0
         for b, c in mine:
             assert b == at and c > 0
             at += c
-            assert (b + c - 1) // page - b // page + 1 <= 1024
+            assert (b + c - 1) // page - b // page + 1 <= 256
         assert at == n
 
 
