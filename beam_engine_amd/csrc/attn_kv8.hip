@@ -40,11 +40,11 @@ template <typename T, bool HIGH> __device__ __forceinline__ uint32_t value2(int 
   else
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, HIGH));
 }
-// Eight codes without a scale.
-template <typename T> __device__ __forceinline__ v8s codes8(int a, int b) {
+// Eight codes times the scale.
+template <typename T> __device__ __forceinline__ v8s codes8(int a, int b, float scale = 1.f) {
   typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(v8s, (u4){value2<T, false>(a, 1.f), value2<T, true>(a, 1.f), value2<T, false>(b, 1.f),
-                                      value2<T, true>(b, 1.f)});
+  return __builtin_bit_cast(v8s, (u4){value2<T, false>(a, scale), value2<T, true>(a, scale), value2<T, false>(b, scale),
+                                      value2<T, true>(b, scale)});
 }
 // Two codes under a scale each.
 template <typename T, bool HIGH> __device__ __forceinline__ uint32_t value11(int codes, float s0, float s1) {
@@ -109,23 +109,30 @@ __device__ __forceinline__ void dma_byte(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
 }
 
+// 16 bytes a lane from a wave-uniform base and a byte offset, as stream::dma16_sv.
+__device__ __forceinline__ void dma16_s(uint64_t base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+
 // An item's pages: ids and scale bytes to LDS, and the K and V codes of its tiles,
 // global -> LDS directly.  The chain of a workgroup's start is three round trips: the
 // item's record, page ids (with Q), scales and the first tiles.  The scales leave ahead
 // of the tiles, so a wait for the first tile is one for them.
 //
-// PAGED: pages hold whole loads' rows (1 KB), so a load's page is wave-uniform: its id
-// comes from a register (64 of the item's ids) by v_readlane and its address is scalar.
-// Otherwise every lane looks its row's page up in LDS.  Past the item's end K re-reads
-// its last token (the scores are masked) and V reads zeros.
-template <int D, bool PAGED, int (*SWZ)(int)>
+// PG 2: page sizes that are multiples of 16, the rows a wave loads of a tile: one page,
+// whose id comes from a register (64 of the item's ids) by v_readlane, and a scalar
+// address.  PG 1: multiples of a load's rows (1 KB), each load's page so.  PG 0: every
+// lane looks its row's page up in LDS.  Past the item's end K re-reads its last token
+// (the scores are masked) and V reads zeros.
+template <int D, int PG, int (*SWZ)(int)>
 struct Codes {
+  static constexpr bool PAGED = PG > 0;
   static constexpr int CPR = D / 16, RPI = 64 / CPR;   // 16-byte chunks per row, rows per wave load
   static constexpr int IPW = kTile / RPI / 4;          // loads per wave per tile (K and V each)
   static constexpr int PLANE = kTile * D, STAGE = 2 * PLANE;
 
   uint64_t kvb;
-  uint32_t row_bytes, page_bytes, vplane, off;
+  uint32_t row_bytes, page_bytes, vplane, off[IPW];
   int w, lane, ps, tok_count, slot0, n_pages, tok;
   float inv_ps;
   int page[IPW], slot[IPW], dpage, dslot;              // PAGED: of the next tile's loads
@@ -155,15 +162,18 @@ struct Codes {
     kvb = reinterpret_cast<uint64_t>(a.kv) + (uint64_t)kvh * D;
     tok = 0;
     pg_base = 0;
-    // (the swizzle of a load's rows: r0 + lane / CPR differs from lane / CPR by a multiple of RPI)
-    off = (uint32_t)(lane / CPR) * row_bytes;
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) {
+      const int lr = lane / CPR;
+      off[i] = (uint32_t)((PG == 2 ? i * RPI : 0) + lr) * row_bytes + ((uint32_t)((lane % CPR) ^ SWZ((w * IPW + i) * RPI + lr)) << 4);
+    }
     if constexpr (PAGED) {
-      dpage = (int)(((float)kTile + 0.5f) * inv_ps);
+      dpage = rfl((int)(((float)kTile + 0.5f) * inv_ps));
       dslot = kTile - dpage * ps;
 #pragma unroll
-      for (int i = 0; i < IPW; ++i) {
+      for (int i = 0; i < (PG == 2 ? 1 : IPW); ++i) {
         const int t = slot0 + (w * IPW + i) * RPI;
-        page[i] = (int)(((float)t + 0.5f) * inv_ps);
+        page[i] = rfl((int)(((float)t + 0.5f) * inv_ps));
         slot[i] = t - page[i] * ps;
       }
     }
@@ -179,54 +189,66 @@ struct Codes {
     if constexpr (!PAGED) __syncthreads();
   }
 
-  template <bool WHOLE>
-  __device__ __forceinline__ void rows(uint32_t dst0) {
+  // Scalar address of a row of the wave's pages.
+  __device__ __forceinline__ uint64_t base_of(int pg, int sl) const {
+    const uint32_t pid = (uint32_t)__builtin_amdgcn_readlane(pg_reg, pg - pg_base);
+    return kvb + (uint64_t)pid * page_bytes + (uint32_t)sl * row_bytes;
+  }
+  __device__ __forceinline__ void advance(int i) {
+    slot[i] += dslot;
+    const bool carry = slot[i] >= ps;
+    slot[i] -= carry ? ps : 0;
+    page[i] += dpage + (carry ? 1 : 0);
+  }
+
+  __device__ __forceinline__ void whole(uint32_t dst0) {
+    dst0 += w * IPW * 1024;
+    if constexpr (PG == 2) {
+      const uint64_t base = base_of(page[0], slot[0]);
+#pragma unroll
+      for (int i = 0; i < IPW; ++i) dma16_s(base, off[i], dst0 + i * 1024);
+#pragma unroll
+      for (int i = 0; i < IPW; ++i) dma16_s(base + vplane, off[i], dst0 + i * 1024 + PLANE);
+      advance(0);
+    } else if constexpr (PG == 1) {
+#pragma unroll
+      for (int i = 0; i < IPW; ++i) {
+        const uint64_t base = base_of(page[i], slot[i]);
+        dma16_s(base, off[i], dst0 + i * 1024);
+        dma16_s(base + vplane, off[i], dst0 + i * 1024 + PLANE);
+        advance(i);
+      }
+    } else {
+      any(dst0);
+    }
+  }
+  // Any tile, row by row.
+  __device__ __forceinline__ void any(uint32_t dst) {
 #pragma unroll
     for (int i = 0; i < IPW; ++i) {
-      const int r0 = (w * IPW + i) * RPI, lr = lane / CPR;
-      const uint32_t dst = dst0 + (w * IPW + i) * 1024, ch = (uint32_t)((lane % CPR) ^ SWZ(r0 + lr)) << 4;
-      const int left = tok_count - 1 - (tok + r0);     // rows of this load up to the item's last token
-      if constexpr (PAGED) {
-        int pg = page[i], sl = slot[i];
-        if (!WHOLE && left < 0) {                      // the load lies past the end: the last token's row
-          pg = n_pages - 1;
-          sl = slot0 + tok_count - 1 - pg * ps;
-        }
-        const uint32_t pid = (uint32_t)__builtin_amdgcn_readlane(pg_reg, pg - pg_base);
-        const uint64_t base = kvb + (uint64_t)pid * page_bytes + (uint32_t)sl * row_bytes;
-        const uint32_t o = (WHOLE ? off : (uint32_t)min(lr, max(left, 0)) * row_bytes) + ch;
-        stream::dma16_sv(base, o, dst);
-        if constexpr (WHOLE) {
-          stream::dma16_sv(base + vplane, o, dst + PLANE);
-        } else {
-          stream::dma16(lr <= left ? reinterpret_cast<const void*>(base + vplane + o) : &kZeroChunk, dst + PLANE);
-        }
-        slot[i] += dslot;
-        const bool carry = slot[i] >= ps;
-        slot[i] -= carry ? ps : 0;
-        page[i] += dpage + (carry ? 1 : 0);
-      } else {
-        const bool in = WHOLE || lr <= left;
-        const int t = in ? tok + r0 + lr : tok_count - 1, pg = page_of(t), sl = slot0 + t - pg * ps;
-        const uint64_t src = kvb + (uint64_t)(uint32_t)pg_lds[pg] * page_bytes + (uint32_t)sl * row_bytes + ch;
-        stream::dma16(reinterpret_cast<const void*>(src), dst);
-        stream::dma16(in ? reinterpret_cast<const void*>(src + vplane) : &kZeroChunk, dst + PLANE);
-      }
+      const int r = (w * IPW + i) * RPI + lane / CPR;
+      const bool in = tok + r < tok_count;
+      const int t = in ? tok + r : tok_count - 1, pg = page_of(t), sl = slot0 + t - pg * ps;
+      const uint32_t pid = PAGED ? (uint32_t)__shfl(pg_reg, pg - pg_base) : (uint32_t)pg_lds[pg];
+      const uint64_t src = kvb + (uint64_t)pid * page_bytes + (uint32_t)sl * row_bytes + ((uint32_t)((lane % CPR) ^ SWZ(r)) << 4);
+      stream::dma16(reinterpret_cast<const void*>(src), dst + i * 1024);
+      stream::dma16(in ? reinterpret_cast<const void*>(src + vplane) : &kZeroChunk, dst + i * 1024 + PLANE);
     }
   }
 
   // The next tile's loads, to LDS byte address dst0 (2 IPW vector memory operations).
   __device__ __forceinline__ void load(uint32_t dst0) {
     if constexpr (PAGED) {
-      // (a tile's pages lie within 64 of its first; pg_lds is read from the third tile on,
-      // behind a barrier: the first two lie within the register's first 64 pages)
-      if (min(page[IPW - 1], n_pages - 1) - pg_base >= 64) {
-        pg_base = min(page[0], n_pages - 1);
-        pg_reg = pg_lds[min(pg_base + lane, n_pages - 1)];
+      // (the wave's pages of a tile lie within 64 of its first; pg_lds is read from the third
+      // tile on, behind a barrier: the first two lie within the register's first 64 pages)
+      const int last = n_pages - 1, p1 = min(page[PG == 2 ? 0 : IPW - 1], last);
+      if (p1 - pg_base >= 64) {
+        pg_base = min(page[0], last);
+        pg_reg = pg_lds[min(pg_base + lane, last)];
       }
     }
-    if (__builtin_expect(tok + kTile <= tok_count, 1)) rows<true>(dst0);
-    else rows<false>(dst0);
+    if (__builtin_expect(tok + kTile <= tok_count, 1)) whole(dst0);
+    else any(dst0 + w * IPW * 1024);
     tok += kTile;
   }
 
@@ -240,10 +262,10 @@ struct Codes {
   }
 };
 
-template <typename T, int D, int RT, bool PAGED, bool QUADS>
+template <typename T, int D, int RT, int PG, bool QUADS>
 __device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& it, TileShared<D>& sh) {
   constexpr int CPR = D / 16;                        // 16-code chunks of a row
-  using Loader = Codes<D, PAGED, swz<CPR>>;
+  using Loader = Codes<D, PG, swz<CPR>>;
   constexpr int PLANE = Loader::PLANE, STAGE = Loader::STAGE, NST = TileShared<D>::kStages;
   constexpr int KP = D / 64;                         // K chunk quads: two QK contraction steps each
   constexpr int TS = RT == 4 ? 1 : 2;                // waves sharing a row tile: token halves,
@@ -506,15 +528,18 @@ __device__ __forceinline__ int swz32(int r) {
 // of a 32-token Sᵀ block (lane l: row l % 32, tokens 8 (i / 4) + 4 (l / 32) + i % 4) is,
 // eight registers at a time, the B operand of Oᵀ += Vᵀ Pᵀ over the token order that the
 // transposed V reads follow.
-template <typename T, int D, int RT, bool PAGED, bool QUADS>
+template <typename T, int D, int RT, int PG, bool QUADS>
 __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& it, TileShared<D>& sh) {
   constexpr int CPR = D / 16;                        // 16-code chunks of a row
-  using Loader = Codes<D, PAGED, swz32<CPR>>;
+  using Loader = Codes<D, PG, swz32<CPR>>;
   constexpr int PLANE = Loader::PLANE, STAGE = Loader::STAGE, NST = TileShared<D>::kStages;
   constexpr int KP = D / 32;                         // K chunk pairs: two QK contraction steps each
   constexpr int CS = RT == 1 ? 2 : 1;
   constexpr int MB = D / 32 / CS;                    // Oᵀ head_dim blocks of a wave
   constexpr int COMB_SLOT = (MB * 16 * 64 + 2 * 64) * 4;
+  // bf16: K's scale in its conversion (every lane holds one token's codes); fp16, whose
+  // values it could take out of range, on the fp32 scores
+  constexpr bool POST = std::is_same<T, f16_t>::value;
   static_assert(2 * COMB_SLOT <= NST * STAGE && RT * 32 * D * 4 <= NST * STAGE, "scratch must fit");
 
   unsigned char* stage = sh.stage;
@@ -540,6 +565,11 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
     const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(it.q_begin + j) * a.q_sn + (int64_t)(kvh * g + hh) * a.q_sh;
 #pragma unroll
     for (int x = 0; x < 2 * KP; ++x) qf[x] = *reinterpret_cast<const v8s*>(qp + 16 * (2 * (x >> 1) + h) + 8 * (x & 1));
+    // (the max is of unscaled scores: a negative scale moves its sign into Q, a zero one zeroes Q)
+    if (!POST && a.scale_log2 <= 0.f) {
+#pragma unroll
+      for (int x = 0; x < 2 * KP; ++x) qf[x] = a.scale_log2 == 0.f ? (v8s)(short)0 : qf[x] ^ (v8s)(short)0x8000;
+    }
   } else {
 #pragma unroll
     for (int x = 0; x < 2 * KP; ++x) qf[x] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
@@ -567,7 +597,8 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
   for (int mb = 0; mb < MB; ++mb)
     voff[mb] = vr * D + (((2 * (cs * MB + mb) + ((lane >> 4) & 1)) ^ swz32<CPR>(vr)) << 4) + (lane & 1) * 8;
 
-  float m_run = -INFINITY, l_run = 0.f;
+  const float scale = POST || a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
+  float m_run = -INFINITY, l_run = 0.f;              // the sums' reference (times `scale`), the weights' sum
   v16f o_acc[MB];
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb)
@@ -588,14 +619,26 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
     if (!active || s0 >= it.tok_count) continue;
     const unsigned char* kt = stage + st * STAGE + ts * 32 * D;
     const unsigned char* vt = kt + PLANE;
-    // scales of the lane's tokens, quad 8 q + 4 h .. + 3 or one each
+    // scales: K of the lane's row, or (POST) K, and V, of its tokens in the C layout,
+    // quad 8 i + 4 h .. + 3 or one each
     constexpr int NS = QUADS ? 4 : 16;
-    float ks[NS], vs[NS];
+    auto token = [&](int i) { return s0 + (QUADS ? 8 * i + 4 * h : 8 * (i >> 2) + 4 * h + (i & 3)); };
+    float kr = 1.f, ks[POST ? NS : 1], vs[NS];
+    if constexpr (!POST) kr = __uint_as_float(sh.ks[ld.page_of(s0 + lr)] << 23);
+    if constexpr (PG == 2) {                         // 16 tokens: one page
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int pg = ld.page_of(s0 + (QUADS ? 8 * i + 4 * h : 8 * (i >> 2) + 4 * h + (i & 3)));
-      ks[i] = __uint_as_float(sh.ks[pg] << 23) * a.scale_log2;
-      vs[i] = __uint_as_float(sh.vs[pg] << 23);
+      for (int i = 0; i < 4; i += 2) {
+        const int pg = ld.page_of(s0 + 8 * i);
+        if constexpr (POST) ks[i] = ks[i + 1] = __uint_as_float(sh.ks[pg] << 23) * a.scale_log2;
+        vs[i] = vs[i + 1] = __uint_as_float(sh.vs[pg] << 23);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const int pg = ld.page_of(token(i));
+        if constexpr (POST) ks[i] = __uint_as_float(sh.ks[pg] << 23) * a.scale_log2;
+        vs[i] = __uint_as_float(sh.vs[pg] << 23);
+      }
     }
     v16f x;
 #pragma unroll
@@ -605,11 +648,13 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
     for (int kp = 0; kp < KP; ++kp) kc[kp] = *reinterpret_cast<const v4i*>(kt + koff[kp]);
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
-      x = mfma32<T>(codes8<T>(kc[kp][0], kc[kp][1]), qf[2 * kp], x);
-      x = mfma32<T>(codes8<T>(kc[kp][2], kc[kp][3]), qf[2 * kp + 1], x);
+      x = mfma32<T>(codes8<T>(kc[kp][0], kc[kp][1], kr), qf[2 * kp], x);
+      x = mfma32<T>(codes8<T>(kc[kp][2], kc[kp][3], kr), qf[2 * kp + 1], x);
     }
+    if constexpr (POST) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] *= ks[QUADS ? i >> 2 : i];
+      for (int i = 0; i < 16; ++i) x[i] *= ks[QUADS ? i >> 2 : i];
+    }
     if (__builtin_amdgcn_ballot_w64(lim < s0 + 32) != 0) {
       const int left = lim - s0 - 4 * h;
 #pragma unroll
@@ -619,22 +664,25 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
     float mx = x[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
-    mx = other_half(mx, false);
-    const float m_new = fmaxf(m_run, mx);
-    const float msafe = m_new == -INFINITY ? 0.f : m_new;
-    if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0) {
-      const float alpha = __builtin_amdgcn_exp2f(m_run - msafe);      // 0 while nothing was seen
+    mx = other_half(mx, false) * scale;
+    // The reference follows when a row's largest score is 2^8 ahead of it (weights, their
+    // sum and Oᵀ are fp32 or of 8 bits' more range): most tiles rescale nothing
+    if (__builtin_amdgcn_ballot_w64(mx > m_run + 8.f) != 0) {
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));   // 0 while nothing was seen
       l_run *= alpha;
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) o_acc[mb] *= alpha;
+      m_run = m_new;
     }
-    m_run = m_new;
+    const float msafe = m_run == -INFINITY ? 0.f : m_run;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       uint32_t pw[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p0 = __builtin_amdgcn_exp2f(x[8 * s + 2 * i] - msafe), p1 = __builtin_amdgcn_exp2f(x[8 * s + 2 * i + 1] - msafe);
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(x[8 * s + 2 * i], scale, -msafe));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(x[8 * s + 2 * i + 1], scale, -msafe));
         l_run += p0 + p1;
         pw[i] = stream::pack2<T>(p0, p1);
       }
@@ -683,14 +731,14 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
       const float cb = (M == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(mb_ - M);
       l_run = l_run * ca + lb * cb;
       m_run = M;
-      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      const float inv = l_run > 0.f ? 1.f / l_run : 0.f, fa = ca * inv, fb = cb * inv;
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const v4f v = *reinterpret_cast<const v4f*>(slot + ((mb * 4 + i) * 64 + lane) * 4);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o_acc[mb][4 * i + e] = (o_acc[mb][4 * i + e] * ca + v[e] * cb) * inv;
+          for (int e = 0; e < 4; ++e) o_acc[mb][4 * i + e] = fmaf(v[e], fb, o_acc[mb][4 * i + e] * fa);
         }
       if (sh.nan_any) {
 #pragma unroll
@@ -733,7 +781,7 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
 
 // A workgroup takes as many row tiles as its item has: with fewer, the waves share out
 // the tokens of a row tile (and the columns) rather than idle.
-template <typename T, int D, bool PAGED, bool QUADS>
+template <typename T, int D, int PG, bool QUADS>
 __global__ __launch_bounds__(256, D == 256 || !QUADS ? 2 : D == 128 ? 3 : 4) void attn_kv8_kernel(AttnArgs a, int first_item) {
   __shared__ __attribute__((aligned(1024))) TileShared<D> sh;
   const int item = first_item + (int)blockIdx.x;
@@ -741,13 +789,13 @@ __global__ __launch_bounds__(256, D == 256 || !QUADS ? 2 : D == 128 ? 3 : 4) voi
   const WorkItem it = a.items[item];
   const int R = it.q_count * a.g;
   if (R <= 16) {
-    tile_item<T, D, 1, PAGED, QUADS>(a, it, sh);
+    tile_item<T, D, 1, PG, QUADS>(a, it, sh);
   } else if constexpr (D == 256) {                   // (32-row tiles would not fit the registers)
-    if (R <= 32) tile_item<T, D, 2, PAGED, QUADS>(a, it, sh);
-    else tile_item<T, D, 4, PAGED, QUADS>(a, it, sh);
+    if (R <= 32) tile_item<T, D, 2, PG, QUADS>(a, it, sh);
+    else tile_item<T, D, 4, PG, QUADS>(a, it, sh);
   } else {
-    if (R <= 32) tile32_item<T, D, 1, PAGED, QUADS>(a, it, sh);
-    else tile32_item<T, D, 2, PAGED, QUADS>(a, it, sh);
+    if (R <= 32) tile32_item<T, D, 1, PG, QUADS>(a, it, sh);
+    else tile32_item<T, D, 2, PG, QUADS>(a, it, sh);
   }
 }
 
@@ -756,9 +804,10 @@ static int launch_tile(const be_attn_plan_info* info, const AttnArgs& a, hipStre
   const int first = info->num_wg;                    // items of more than 64 rows come first
   const dim3 grid(info->grid_items - first, info->num_kv_heads);
   if (grid.x == 0) return BE_OK;
-  if (paged4(a.page_size, D) && a.page_size % 4 == 0) attn_kv8_kernel<T, D, true, true><<<grid, 256, 0, st>>>(a, first);
-  else if (a.page_size % 4 == 0) attn_kv8_kernel<T, D, false, true><<<grid, 256, 0, st>>>(a, first);
-  else attn_kv8_kernel<T, D, false, false><<<grid, 256, 0, st>>>(a, first);
+  if (a.page_size % 16 == 0) attn_kv8_kernel<T, D, 2, true><<<grid, 256, 0, st>>>(a, first);
+  else if (paged4(a.page_size, D)) attn_kv8_kernel<T, D, 1, true><<<grid, 256, 0, st>>>(a, first);
+  else if (a.page_size % 4 == 0) attn_kv8_kernel<T, D, 0, true><<<grid, 256, 0, st>>>(a, first);
+  else attn_kv8_kernel<T, D, 0, false><<<grid, 256, 0, st>>>(a, first);
   BE_HIP_CHECK(hipGetLastError());
   return BE_OK;
 }
