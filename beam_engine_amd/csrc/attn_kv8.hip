@@ -536,11 +536,11 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
   constexpr int KP = D / 32;                         // K chunk pairs: two QK contraction steps each
   constexpr int CS = RT == 1 ? 2 : 1;
   constexpr int MB = D / 32 / CS;                    // Oᵀ head_dim blocks of a wave
-  constexpr int COMB_SLOT = (MB * 16 * 64 + 2 * 64) * 4;
+  constexpr int COMB_SLOT = (MB * 8 * 64 + 2 * 64) * 4;
   // bf16: K's scale in its conversion (every lane holds one token's codes); fp16, whose
   // values it could take out of range, on the fp32 scores
   constexpr bool POST = std::is_same<T, f16_t>::value;
-  static_assert(2 * COMB_SLOT <= NST * STAGE && RT * 32 * D * 4 <= NST * STAGE, "scratch must fit");
+  static_assert(4 * COMB_SLOT <= NST * STAGE, "combine scratch must fit");
 
   unsigned char* stage = sh.stage;
   const int kvh = blockIdx.y;
@@ -643,13 +643,11 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
     v16f x;
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = 0.f;
-    v4i kc[KP];
-#pragma unroll
-    for (int kp = 0; kp < KP; ++kp) kc[kp] = *reinterpret_cast<const v4i*>(kt + koff[kp]);
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
-      x = mfma32<T>(codes8<T>(kc[kp][0], kc[kp][1], kr), qf[2 * kp], x);
-      x = mfma32<T>(codes8<T>(kc[kp][2], kc[kp][3], kr), qf[2 * kp + 1], x);
+      const v4i kc = *reinterpret_cast<const v4i*>(kt + koff[kp]);
+      x = mfma32<T>(codes8<T>(kc[0], kc[1], kr), qf[2 * kp], x);
+      x = mfma32<T>(codes8<T>(kc[2], kc[3], kr), qf[2 * kp + 1], x);
     }
     if constexpr (POST) {
 #pragma unroll
@@ -707,76 +705,56 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
   }
   l_run = other_half(l_run, true);
 
-  // ---- the second token half hands its state to the first
-  float* comb = reinterpret_cast<float*>(stage);
-  {
-    float* slot = comb + (RT == 1 ? cs : rt) * (COMB_SLOT / 4);
-    __syncthreads();                                   // tiles no longer needed
-    if (ts > 0 && active) {
+  // ---- the two token halves exchange half of their columns and each finishes its own
+  const int pair = RT == 1 ? cs : rt;
+  float* give = reinterpret_cast<float*>(stage) + (2 * pair + ts) * (COMB_SLOT / 4);
+  const float* take = reinterpret_cast<const float*>(stage) + (2 * pair + (ts ^ 1)) * (COMB_SLOT / 4);
+  constexpr int HB = MB * 4 / 2;                     // v4f groups (mb, i) of a half
+  auto group = [&](int q) { return v4f{o_acc[q >> 2][4 * (q & 3)], o_acc[q >> 2][4 * (q & 3) + 1], o_acc[q >> 2][4 * (q & 3) + 2], o_acc[q >> 2][4 * (q & 3) + 3]}; };
+  __syncthreads();                                   // tiles no longer needed
+  if (active) {
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v4f v = {o_acc[mb][4 * i], o_acc[mb][4 * i + 1], o_acc[mb][4 * i + 2], o_acc[mb][4 * i + 3]};
-          *reinterpret_cast<v4f*>(slot + ((mb * 4 + i) * 64 + lane) * 4) = v;
-        }
-      slot[MB * 1024 + lane] = m_run;
-      slot[MB * 1024 + 64 + lane] = l_run;
-    }
-    __syncthreads();
-    if (ts == 0 && active) {
-      const float mb_ = slot[MB * 1024 + lane], lb = slot[MB * 1024 + 64 + lane];
-      const float M = fmaxf(m_run, mb_);
-      const float ca = (M == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(m_run - M);
-      const float cb = (M == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(mb_ - M);
-      l_run = l_run * ca + lb * cb;
-      m_run = M;
-      const float inv = l_run > 0.f ? 1.f / l_run : 0.f, fa = ca * inv, fb = cb * inv;
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v4f v = *reinterpret_cast<const v4f*>(slot + ((mb * 4 + i) * 64 + lane) * 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o_acc[mb][4 * i + e] = fmaf(v[e], fb, o_acc[mb][4 * i + e] * fa);
-        }
-      if (sh.nan_any) {
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (sh.nan_tok[32 * (cs * MB + mb) + 8 * (i >> 2) + 4 * h + (i & 3)] < lim) o_acc[mb][i] = NAN;
-      }
-      if (h == 0 && cs == 0 && row < R) store_lse(a, it, j, kvh * g + hh, m_run, l_run);
-    }
-    __syncthreads();                                   // the states have been read
-  }
-
-  // ---- writes, through LDS so that they are whole rows: lane holds
-  // Oᵀ[32 (cs MB + mb) + 8 (i / 4) + 4 h + i % 4][row]; rows of D floats, 16-byte chunk c at c ^ (row & 15)
-  if (ts == 0 && active) {
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const v4f v = {o_acc[mb][4 * i], o_acc[mb][4 * i + 1], o_acc[mb][4 * i + 2], o_acc[mb][4 * i + 3]};
-        *reinterpret_cast<v4f*>(comb + row * D + (((8 * (cs * MB + mb) + 2 * i + h) ^ (row & 15)) << 2)) = v;
-      }
+    for (int q = 0; q < HB; ++q) *reinterpret_cast<v4f*>(give + (q * 64 + lane) * 4) = ts ? group(q) : group(HB + q);
+    give[HB * 256 + lane] = m_run;
+    give[HB * 256 + 64 + lane] = l_run;
   }
   __syncthreads();
+  if (!active) return;
+  const float mb_ = take[HB * 256 + lane], lb = take[HB * 256 + 64 + lane];
+  const float M = fmaxf(m_run, mb_);
+  const float ca = (M == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(m_run - M);
+  const float cb = (M == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(mb_ - M);
+  l_run = l_run * ca + lb * cb;
+  const float inv = l_run > 0.f ? 1.f / l_run : 0.f, fa = ca * inv, fb = cb * inv;
+  v4f y[HB];
 #pragma unroll
-  for (int c0 = 0; c0 < RT * 32 * (D / 4); c0 += 256) {
-    const int r = (c0 + tid) / (D / 4), ch = tid % (D / 4);
-    if (r >= R) break;
-    const int rj = (int)(((float)r + 0.5f) * (1.f / (float)g)), head = kvh * g + r - rj * g;
-    const v4f v = *reinterpret_cast<const v4f*>(comb + r * D + ((ch ^ (r & 15)) << 2));
-    if (it.out_row < 0) {
-      T* op = reinterpret_cast<T*>(a.out) + (int64_t)(it.q_begin + rj) * a.o_sn + (int64_t)head * a.o_sh;
-      *reinterpret_cast<v4s*>(op + 4 * ch) = pack4<T>(v[0], v[1], v[2], v[3]);
-    } else {
-      *reinterpret_cast<v4f*>(a.part_o + ((int64_t)(it.out_row + rj) * a.hq + head) * D + 4 * ch) = v;
-    }
+  for (int q = 0; q < HB; ++q) {
+    const v4f v = *reinterpret_cast<const v4f*>(take + (q * 64 + lane) * 4), mine = ts ? group(HB + q) : group(q);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[q][e] = fmaf(v[e], fb, mine[e] * fa);
   }
+  // lane holds Oᵀ[d0 + 32 (q / 4) + 8 (q % 4) .. + 3][row]
+  const int d0 = 32 * cs * MB + (ts * HB / 4) * 32 + 4 * h, head = kvh * g + hh;
+  static_assert(HB % 4 == 0 || MB == 1, "a half is whole blocks, or half of one");
+  const int q0 = MB == 1 ? ts * HB : 0;              // (one block: the half's first quad)
+  if (sh.nan_any) {
+#pragma unroll
+    for (int q = 0; q < HB; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (sh.nan_tok[d0 + 32 * (q >> 2) + 8 * ((q0 + q) & 3) + e] < lim) y[q][e] = NAN;
+  }
+  if (row >= R) return;
+  if (it.out_row < 0) {
+    T* op = reinterpret_cast<T*>(a.out) + (int64_t)(it.q_begin + j) * a.o_sn + (int64_t)head * a.o_sh + d0;
+#pragma unroll
+    for (int q = 0; q < HB; ++q) *reinterpret_cast<v4s*>(op + 32 * (q >> 2) + 8 * ((q0 + q) & 3)) = pack4<T>(y[q][0], y[q][1], y[q][2], y[q][3]);
+  } else {
+    float* op = a.part_o + ((int64_t)(it.out_row + j) * a.hq + head) * D + d0;
+#pragma unroll
+    for (int q = 0; q < HB; ++q) *reinterpret_cast<v4f*>(op + 32 * (q >> 2) + 8 * ((q0 + q) & 3)) = y[q];
+  }
+  if (h == 0 && cs == 0 && ts == 0) store_lse(a, it, j, head, M, l_run);
 }
 
 // A workgroup takes as many row tiles as its item has: with fewer, the waves share out
