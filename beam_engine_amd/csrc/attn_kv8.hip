@@ -133,7 +133,7 @@ struct Codes {
 
   uint64_t kvb;
   uint32_t row_bytes, page_bytes, vplane, off[IPW];
-  int w, lane, ps, tok_count, slot0, n_pages, tok;
+  int tid, w, lane, ps, tok_count, slot0, n_pages, tok;
   float inv_ps;
   int page[IPW], slot[IPW], dpage, dslot;              // PAGED: of the next tile's loads
   int id, pg_reg, pg_base;
@@ -145,16 +145,17 @@ struct Codes {
   }
 
   // The page ids leave; nothing waits for them yet.
-  __device__ __forceinline__ void begin(const AttnArgs& a, const WorkItem& it, int kvh, int wave) {
-    w = wave;
-    lane = threadIdx.x & 63;
+  __device__ __forceinline__ void begin(const AttnArgs& a, const WorkItem& it, int kvh, int thread) {
+    tid = thread;
+    w = rfl(tid >> 6);
+    lane = tid & 63;
     ps = a.page_size;
     inv_ps = 1.f / (float)ps;
     tok_count = it.tok_count;
     slot0 = it.tok_begin - it.first_page * ps;
     n_pages = (int)(((float)(slot0 + tok_count - 1) + 0.5f) * inv_ps) + 1;
     const int32_t* pages = a.pages + it.page_begin + it.first_page;
-    id = pages[min((int)threadIdx.x, n_pages - 1)];
+    id = pages[min(tid, n_pages - 1)];
     pg_reg = PAGED ? pages[min(lane, n_pages - 1)] : 0;
     row_bytes = (uint32_t)a.hkv * D;
     vplane = (uint32_t)ps * row_bytes;
@@ -181,7 +182,7 @@ struct Codes {
 
   // Ids to LDS, scales on their way there.
   __device__ __forceinline__ void stage(const AttnArgs& a, int kvh, int32_t* pg, uint32_t* ks, uint32_t* vs) {
-    pg[threadIdx.x] = id;
+    pg[tid] = id;
     pg_lds = pg;
     const uint8_t* sc = a.kv_scale + (int64_t)id * 2 * a.hkv + kvh;
     dma_byte(sc, lds_addr(ks) + w * 256);
@@ -262,8 +263,16 @@ struct Codes {
   }
 };
 
+// The item in each of a kernel's branches by itself: what they share would otherwise be
+// computed ahead of them and held (spilled) for all of them.
+__device__ __forceinline__ WorkItem opaque(WorkItem it) {
+  asm volatile("" : "+s"(it.page_begin), "+s"(it.tok_begin), "+s"(it.tok_count), "+s"(it.first_page), "+s"(it.q_begin), "+s"(it.q_count));
+  return it;
+}
+
 template <typename T, int D, int RT, int PG, bool QUADS>
-__device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& it, TileShared<D>& sh) {
+__device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& item, TileShared<D>& sh) {
+  const WorkItem it = opaque(item);
   constexpr int CPR = D / 16;                        // 16-code chunks of a row
   using Loader = Codes<D, PG, swz<CPR>>;
   constexpr int PLANE = Loader::PLANE, STAGE = Loader::STAGE, NST = TileShared<D>::kStages;
@@ -278,13 +287,14 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& it,
   unsigned char* stage = sh.stage;
   int32_t* nan_tok = sh.nan_tok;
   const int kvh = blockIdx.y;
-  const int tid = threadIdx.x;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
   const int w = rfl(tid >> 6), lane = tid & 63, lg = lane >> 4, lc = lane & 15;
   const int g = a.g, R = it.q_count * g;
   const int n_tiles = (it.tok_count + kTile - 1) / kTile;
   const uint32_t lds0 = lds_addr(stage);
   Loader ld;
-  ld.begin(a, it, kvh, w);
+  ld.begin(a, it, kvh, tid);
 
   // ---- wave role
   const int rt = RT == 1 ? 0 : w % RT, ts = RT == 4 ? 0 : RT == 2 ? w >> 1 : w & 1, cs = RT == 1 ? w >> 1 : 0;
@@ -529,7 +539,8 @@ __device__ __forceinline__ int swz32(int r) {
 // eight registers at a time, the B operand of Oᵀ += Vᵀ Pᵀ over the token order that the
 // transposed V reads follow.
 template <typename T, int D, int RT, int PG, bool QUADS>
-__device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& it, TileShared<D>& sh) {
+__device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& item, TileShared<D>& sh) {
+  const WorkItem it = opaque(item);
   constexpr int CPR = D / 16;                        // 16-code chunks of a row
   using Loader = Codes<D, PG, swz32<CPR>>;
   constexpr int PLANE = Loader::PLANE, STAGE = Loader::STAGE, NST = TileShared<D>::kStages;
@@ -544,13 +555,14 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
 
   unsigned char* stage = sh.stage;
   const int kvh = blockIdx.y;
-  const int tid = threadIdx.x;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
   const int w = rfl(tid >> 6), lane = tid & 63, h = lane >> 5, lr = lane & 31;
   const int g = a.g, R = it.q_count * g;
   const int n_tiles = (it.tok_count + kTile - 1) / kTile;
   const uint32_t lds0 = lds_addr(stage);
   Loader ld;
-  ld.begin(a, it, kvh, w);
+  ld.begin(a, it, kvh, tid);
 
   // ---- wave role
   const int rt = RT == 1 ? 0 : w & 1, ts = RT == 1 ? w & 1 : w >> 1, cs = RT == 1 ? w >> 1 : 0;
@@ -588,14 +600,11 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
     lim = (int)std::min<int64_t>(it.tok_count, std::max<int64_t>(v, 0));
   }
   const int unseen = (int)std::min<int64_t>(it.tok_count, std::max<int64_t>((int64_t)it.vis0 - it.tok_begin, 0));
-  // ---- operand offsets (the swizzle repeats every 16 rows)
-  uint32_t koff[KP], voff[MB];
-#pragma unroll
-  for (int kp = 0; kp < KP; ++kp) koff[kp] = lr * D + (((2 * kp + h) ^ swz32<CPR>(lr)) << 4);
+  // ---- operand offsets (the swizzle repeats every 16 rows, and stages start on 2 KB: the
+  // chunks of a row differ by an XOR, which costs an instruction and saves the registers)
+  const uint32_t koff = lr * D + ((h ^ swz32<CPR>(lr)) << 4);
   const int vj = (lane & 15) >> 1, vr = (vj >> 2) * 8 + 4 * h + (vj & 3);
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
-    voff[mb] = vr * D + (((2 * (cs * MB + mb) + ((lane >> 4) & 1)) ^ swz32<CPR>(vr)) << 4) + (lane & 1) * 8;
+  const uint32_t voff = vr * D + (((2 * cs * MB + ((lane >> 4) & 1)) ^ swz32<CPR>(vr)) << 4) + (lane & 1) * 8;
 
   const float scale = POST || a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
   float m_run = -INFINITY, l_run = 0.f;              // the sums' reference (times `scale`), the weights' sum
@@ -619,6 +628,11 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
     if (!active || s0 >= it.tok_count) continue;
     const unsigned char* kt = stage + st * STAGE + ts * 32 * D;
     const unsigned char* vt = kt + PLANE;
+    // every LDS read of the tile well ahead of its use: K's codes and the scales, then V's
+    // codes under the softmax
+    v4i kc[KP];
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) kc[kp] = *reinterpret_cast<const v4i*>(kt + (koff ^ (kp << 5)));
     // scales: K of the lane's row, or (POST) K, and V, of its tokens in the C layout,
     // quad 8 i + 4 h .. + 3 or one each
     constexpr int NS = QUADS ? 4 : 16;
@@ -643,12 +657,18 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
     v16f x;
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
-      const v4i kc = *reinterpret_cast<const v4i*>(kt + koff[kp]);
-      x = mfma32<T>(codes8<T>(kc[0], kc[1], kr), qf[2 * kp], x);
-      x = mfma32<T>(codes8<T>(kc[2], kc[3], kr), qf[2 * kp + 1], x);
+      x = mfma32<T>(codes8<T>(kc[kp][0], kc[kp][1], kr), qf[2 * kp], x);
+      x = mfma32<T>(codes8<T>(kc[kp][2], kc[kp][3], kr), qf[2 * kp + 1], x);
     }
+    v2i vc[2][MB];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) vc[s][mb] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i_t)(vt + s * 16 * D + (voff ^ (mb << 5))));
+    __builtin_amdgcn_sched_barrier(0);
     if constexpr (POST) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] *= ks[QUADS ? i >> 2 : i];
@@ -687,16 +707,15 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
       const v8s pf = __builtin_bit_cast(v8s, (u4){pw[0], pw[1], pw[2], pw[3]});
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
-        const v2i vc = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i_t)(vt + s * 16 * D + voff[mb]));
         u4 vv;
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
           if constexpr (QUADS) {
-            vv[2 * o] = value2<T, false>(vc[o], vs[2 * s + o]);
-            vv[2 * o + 1] = value2<T, true>(vc[o], vs[2 * s + o]);
+            vv[2 * o] = value2<T, false>(vc[s][mb][o], vs[2 * s + o]);
+            vv[2 * o + 1] = value2<T, true>(vc[s][mb][o], vs[2 * s + o]);
           } else {
-            vv[2 * o] = value11<T, false>(vc[o], vs[8 * s + 4 * o], vs[8 * s + 4 * o + 1]);
-            vv[2 * o + 1] = value11<T, true>(vc[o], vs[8 * s + 4 * o + 2], vs[8 * s + 4 * o + 3]);
+            vv[2 * o] = value11<T, false>(vc[s][mb][o], vs[8 * s + 4 * o], vs[8 * s + 4 * o + 1]);
+            vv[2 * o + 1] = value11<T, true>(vc[s][mb][o], vs[8 * s + 4 * o + 2], vs[8 * s + 4 * o + 3]);
           }
         }
         o_acc[mb] = mfma32<T>(__builtin_bit_cast(v8s, vv), pf, o_acc[mb]);
@@ -733,8 +752,12 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[q][e] = fmaf(v[e], fb, mine[e] * fa);
   }
-  // lane holds Oᵀ[d0 + 32 (q / 4) + 8 (q % 4) .. + 3][row]
-  const int d0 = 32 * cs * MB + (ts * HB / 4) * 32 + 4 * h, head = kvh * g + hh;
+  // lane holds Oᵀ[d0 + 32 (q / 4) + 8 (q % 4) .. + 3][row] (the row's query and head again,
+  // not held in registers through the tiles)
+  int row_ = row;
+  asm volatile("" : "+v"(row_));
+  const int j_ = (int)(((float)row_ + 0.5f) * (1.f / (float)g)), head = kvh * g + row_ - j_ * g;
+  const int d0 = 32 * cs * MB + (ts * HB / 4) * 32 + 4 * h;
   static_assert(HB % 4 == 0 || MB == 1, "a half is whole blocks, or half of one");
   const int q0 = MB == 1 ? ts * HB : 0;              // (one block: the half's first quad)
   if (sh.nan_any) {
@@ -744,17 +767,17 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
       for (int e = 0; e < 4; ++e)
         if (sh.nan_tok[d0 + 32 * (q >> 2) + 8 * ((q0 + q) & 3) + e] < lim) y[q][e] = NAN;
   }
-  if (row >= R) return;
+  if (row_ >= R) return;
   if (it.out_row < 0) {
-    T* op = reinterpret_cast<T*>(a.out) + (int64_t)(it.q_begin + j) * a.o_sn + (int64_t)head * a.o_sh + d0;
+    T* op = reinterpret_cast<T*>(a.out) + (int64_t)(it.q_begin + j_) * a.o_sn + (int64_t)head * a.o_sh + d0;
 #pragma unroll
     for (int q = 0; q < HB; ++q) *reinterpret_cast<v4s*>(op + 32 * (q >> 2) + 8 * ((q0 + q) & 3)) = pack4<T>(y[q][0], y[q][1], y[q][2], y[q][3]);
   } else {
-    float* op = a.part_o + ((int64_t)(it.out_row + j) * a.hq + head) * D + d0;
+    float* op = a.part_o + ((int64_t)(it.out_row + j_) * a.hq + head) * D + d0;
 #pragma unroll
     for (int q = 0; q < HB; ++q) *reinterpret_cast<v4f*>(op + 32 * (q >> 2) + 8 * ((q0 + q) & 3)) = y[q];
   }
-  if (h == 0 && cs == 0 && ts == 0) store_lse(a, it, j, head, M, l_run);
+  if (h == 0 && cs == 0 && ts == 0) store_lse(a, it, j_, head, M, l_run);
 }
 
 // A workgroup takes as many row tiles as its item has: with fewer, the waves share out
