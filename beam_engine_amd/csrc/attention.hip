@@ -244,6 +244,83 @@ __global__ __launch_bounds__(256) void merge2_kernel(const float* oa, const floa
 }
 
 // ================================================================== host: planner
+// Query tiles and key chunks of an 8-bit cache's plan: the longest items' chain, the CUs'
+// shares of the tiles, partial rows and the merge are weighed against each other for
+// both row limits (tile kernel only, or 128-row blocks for what exceeds 64 rows) and
+// chunks of 1 to 1024 tiles, and the shortest estimate wins.
+struct Kv8Cut {
+  int rows_cap;
+  int64_t chunk;           // tokens
+  double us;
+};
+// Microseconds at head_dim 128 (kv8_scale for others), MI355X: a 64-token tile of a CU's
+// share, the same for a workgroup that has the CU to itself, a workgroup's start and end
+// as latency and as the CU's time; [0] up to 64 rows, [1] blocks.
+constexpr double kKv8Tile[2] = {1.0, 1.35}, kKv8Alone[2] = {0.9, 1.6}, kKv8Start[2] = {5.0, 6.0}, kKv8Wg[2] = {0.8, 1.5};
+constexpr int kKv8Slots[2] = {3, 2};
+static double kv8_scale(int d) { return 0.35 + 0.65 * d / 128; }
+
+template <typename Vis>
+static Kv8Cut kv8_cut(const std::vector<Group>& groups, const Vis& vis, int g, int hq, int hkv, int d, int num_cus, int only_rows) {
+  const double per_d = kv8_scale(d);
+  Kv8Cut best{0, 0, 0};
+  struct Tile {            // query tiles of a plan: 64-token tiles of keys, rows, how many such
+    int64_t tiles;
+    int rows;
+    int64_t n;
+  };
+  for (int rows_cap : {64, kMaxTileRows}) {
+    if ((only_rows && rows_cap != only_rows) || rows_cap > kv8_max_rows(d) || g > rows_cap) continue;
+    const int q_tile = std::max(1, rows_cap / g);
+    std::vector<Tile> qt;
+    int64_t longest = 1;
+    for (const Group& gr : groups) {
+      if (gr.kv_len <= 0) continue;
+      for (int qa = gr.q0; qa < gr.q1; qa += q_tile) {
+        const int qn = std::min(q_tile, gr.q1 - qa);
+        const int64_t t = ceil_div(vis(gr, qa + qn - 1), kTile);
+        if (t == 0) continue;
+        longest = std::max(longest, t);
+        // (the last tile of a group of blocks is a block too)
+        const int rows = std::min(q_tile, gr.q1 - gr.q0) * g;
+        if (!qt.empty() && qt.back().tiles == t && qt.back().rows == rows) ++qt.back().n;
+        else qt.push_back(Tile{t, rows, 1});
+      }
+    }
+    if (qt.empty()) return Kv8Cut{rows_cap, kTile, 0};
+    for (int64_t c = 1; c <= 1024; c = c < 4 ? c + 1 : c * 5 / 4) {
+      double work[2] = {0, 0}, wgs[2] = {0, 0}, part = 0;
+      int64_t chain[2] = {0, 0};
+      bool split = false;
+      for (const Tile& x : qt) {
+        const int k = x.rows > 64;
+        const int64_t nch = ceil_div(x.tiles, c);
+        work[k] += (double)x.tiles * x.n * hkv;
+        wgs[k] += (double)nch * x.n * hkv;
+        chain[k] = std::max(chain[k], std::min(c, x.tiles));
+        if (nch > 1) {
+          split = true;
+          part += (double)nch * x.n * x.rows * hkv * d * 4;
+        }
+      }
+      double us = 3.0;
+      for (int k = 0; k < 2; ++k) {
+        if (wgs[k] == 0) continue;
+        const double per_cu = wgs[k] / num_cus, slots = kKv8Slots[k], tile = kKv8Tile[k] * per_d;
+        const double share = (work[k] * tile + wgs[k] * kKv8Wg[k]) / num_cus + part / 5e6;
+        const double busy = std::min(slots, std::ceil(per_cu));
+        const double line = kKv8Start[k] + chain[k] * std::max(kKv8Alone[k] * per_d, busy * tile);
+        // the last generation of workgroups runs with what it leaves idle
+        us += std::max(share, line) + (per_cu > slots ? 0.5 * kKv8Start[k] : 0.0) + (k == 1 && wgs[0] > 0 ? 2.5 : 0.0);
+      }
+      if (split) us += 3.0 + part / 5e6;
+      if (best.rows_cap == 0 || us < best.us) best = Kv8Cut{rows_cap, c * kTile, us};
+      if (c >= longest) break;
+    }
+  }
+  return best;
+}
+
 int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, int hkv, int d,
               int page_size, int num_pages, int dtype, int flags, int num_cus, const be_plan_caps* caps,
               int32_t* out, int64_t cap, be_attn_plan_info* info) {
@@ -368,8 +445,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
     BE_REQUIRE(caps->max_items >= 0 && caps->max_queries >= num_queries && caps->max_pages >= 0 &&
                    caps->max_merge >= 0 && caps->max_merge_rows >= 0 && caps->max_zero >= 0,
                "bad plan capacities (max_queries %d < %d queries?)", caps->max_queries, num_queries);
-    // (an 8-bit cache: one kernel for every plan of the layout, unless a group needs blocks)
-    if (mfma) rows_cap = std::min(rows_cap, kv8 && g <= 64 ? std::min(tr, 64) : tr);
+    if (mfma) rows_cap = std::min(rows_cap, kv8 ? std::max(tr, 64) : tr);
     // (fp32: never more items than 32-row ones, which capacities were sized for
     // whatever tile_rows said; causal ones cut their keys by their own rows)
     if (f32 && (tr <= 32 || any_causal)) rows_cap = kMaxRows;
@@ -397,6 +473,14 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
     info->flops = flops;
     return BE_OK;
   }
+  int64_t kv8_chunk = 0;
+  if (kv8) {
+    const Kv8Cut cut = kv8_cut(groups, vis, g, hq, hkv, d, num_cus, caps || rows_cap < 64 || g > 64 ? rows_cap : 0);
+    if (cut.rows_cap) {
+      rows_cap = cut.rows_cap;
+      kv8_chunk = cut.chunk;
+    }
+  }
   const int q_tile = std::max(1, rows_cap / g);
   // Causal groups on the block kernel: a workgroup's tiles run one after the
   // other (about 1.5 us each with the CU to itself, 1.05 us per tile of the CU's
@@ -414,7 +498,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   // 9.4 in 4 chunks; after 1000 11.8 and 9.2).
   int64_t causal_chunk = 0, causal_blocks = 0, tiles = 0, queries = 0, span = 0;
   double block_us = 0;
-  if (any_causal && mfma && !less && !caps && rows_cap == kMaxTileRows && block_eligible(dtype, d)) {
+  if (any_causal && mfma && !kv8 && !less && !caps && rows_cap == kMaxTileRows && block_eligible(dtype, d)) {
     int64_t longest = 0;
     int most_rows = 0;
     std::vector<int64_t> tiles_of;                     // of each query tile
@@ -493,6 +577,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   // reading 4 x D bytes per token (bf16 K + V): keep chunks >= 4 x rows tokens
   // so partial traffic stays under ~1/4 of the KV bytes it summarises.
   auto group_chunk = [&](const Group& gr) -> int64_t {
+    if (kv8_chunk > 0) return std::min(less ? INT32_MAX / 64 * 64 : kv8_chunk, chunk_cap);
     if (causal_chunk > 0) return std::min(std::max<int64_t>(causal_chunk, kTile), chunk_cap);
     const int64_t rows = (int64_t)std::min(q_tile, gr.q1 - gr.q0) * g;
     int64_t c = std::max<int64_t>(chunk, ceil_div(4 * rows, 64) * 64);
@@ -531,7 +616,9 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
         // clamping to [0, kv_len]: may be negative), query j of the item sees
         // vis0 + j (the kernel clamps per row); kNoCausal without the mask
         const int vis0 = gr.kv_len - (gr.q1 - gr.q0) + (qa - gr.q0) + 1;
-        WorkItem w{qa, qn, gr.page_base, t0, tc, -1, is_causal(gr) ? vis0 : kNoCausal, kv8 ? t0 / page_size : 0};
+        WorkItem w{qa, qn, gr.page_base, t0, tc, -1, is_causal(gr) ? vis0 : kNoCausal, 0};
+        // (marked while a block's item)
+        if (kv8) w.first_page = std::min(q_tile, gr.q1 - gr.q0) * g > 64 ? ~(t0 / page_size) : t0 / page_size;
         if (!direct) {
           w.out_row = rows;
           for (int j = 0; j < qn; ++j) rows_of[qa + j].push_back(rows + j);
@@ -551,9 +638,11 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   // an 8-bit cache: items of more than 64 rows first, which the block kernel takes
   int block_items = 0;
   if (kv8) {
-    auto big = [&](const WorkItem& w) { return w.q_count * g > 64; };
-    std::stable_partition(items.begin(), items.end(), big);
-    block_items = (int)std::count_if(items.begin(), items.end(), big);
+    // (a block's last, smaller query tiles go with it: alone they would be a launch of a few
+    // long chains behind it)
+    const auto rest = std::stable_partition(items.begin(), items.end(), [](const WorkItem& w) { return w.first_page < 0; });
+    block_items = (int)(rest - items.begin());
+    for (int i = 0; i < block_items; ++i) items[i].first_page = ~items[i].first_page;
   }
 
   // ---- merge list (queries with partial rows: one of a tile whose other queries
@@ -604,6 +693,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   out[kHdrMerge] = (int32_t)merge_q.size();
   out[kHdrZero] = (int32_t)zero_q.size();
   out[kHdrRows] = rows;
+  if (kv8) out[kHdrBlocks] = block_items;
   memcpy(out + off_items, items.data(), n_items * sizeof(WorkItem));
   for (int i = 0; i < num_queries; ++i) out[off_qindex + i] = i;
   {
@@ -636,9 +726,9 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   info->dtype = dtype;
   info->kernel = kv8 ? 4 : blocks ? 2 : mfma ? 1 : 0;
   info->stream_loop = blocks ? kLoopBlocks : 0;
-  info->num_wg = kv8 ? (caps && block_items ? (int)c_items : block_items) : 0;
+  info->num_wg = !kv8 ? 0 : caps && rows_cap > 64 ? (int)c_items : block_items;
   info->tile_rows = !mfma && !f32 ? 0 : blocks ? 128 : caps ? (f32 || kv8 ? rows_cap : caps->tile_rows) : (max_r <= 16 ? 16 : max_r <= 32 ? 32 : max_r <= 64 ? 64 : 128);
-  info->chunk_tokens = (int32_t)std::min<int64_t>(causal_chunk > 0 ? std::min(causal_chunk, chunk_cap) : chunk, INT32_MAX);
+  info->chunk_tokens = (int32_t)std::min<int64_t>(kv8_chunk > 0 ? std::min(kv8_chunk, chunk_cap) : causal_chunk > 0 ? std::min(causal_chunk, chunk_cap) : chunk, INT32_MAX);
   info->plan_ints = (int32_t)off;
   info->off_items = (int32_t)off_items;
   info->off_qindex = (int32_t)off_qindex;
@@ -748,6 +838,7 @@ int attn_run(const be_attn_plan_info* info, const int32_t* plan, void* partials,
   a.merge_ptr = plan + info->off_merge_ptr;
   a.merge_rows = plan + info->off_merge_rows;
   a.live_items = info->static_layout ? plan + kHdrItems : nullptr;
+  a.live_blocks = info->static_layout ? plan + kHdrBlocks : nullptr;
   a.counters = (info->fused_merge && info->num_merge > 0)
                    ? reinterpret_cast<int32_t*>(reinterpret_cast<char*>(partials) + info->counter_offset)
                    : nullptr;

@@ -785,7 +785,7 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
 template <typename T, int D, int PG, bool QUADS>
 __global__ __launch_bounds__(256, D == 256 || !QUADS ? 2 : D == 128 ? 3 : 4) void attn_kv8_kernel(AttnArgs a, int first_item) {
   __shared__ __attribute__((aligned(1024))) TileShared<D> sh;
-  const int item = first_item + (int)blockIdx.x;
+  const int item = (a.live_blocks ? *a.live_blocks : first_item) + (int)blockIdx.x;
   if (a.live_items && item >= *a.live_items) return;
   const WorkItem it = a.items[item];
   const int R = it.q_count * a.g;
@@ -802,8 +802,8 @@ __global__ __launch_bounds__(256, D == 256 || !QUADS ? 2 : D == 128 ? 3 : 4) voi
 
 template <typename T, int D>
 static int launch_tile(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st) {
-  const int first = info->num_wg;                    // items of more than 64 rows come first
-  const dim3 grid(info->grid_items - first, info->num_kv_heads);
+  const int first = info->num_wg;                    // the block kernel's items come first
+  const dim3 grid(info->static_layout ? info->grid_items : info->grid_items - first, info->num_kv_heads);
   if (grid.x == 0) return BE_OK;
   if (a.page_size % 16 == 0) attn_kv8_kernel<T, D, 2, true><<<grid, 256, 0, st>>>(a, first);
   else if (paged4(a.page_size, D)) attn_kv8_kernel<T, D, 1, true><<<grid, 256, 0, st>>>(a, first);
@@ -821,7 +821,8 @@ __device__ __forceinline__ int swz16(int r) {
   return D == 128 ? ((r & 3) << 2 | ((r >> 2) & 3)) : (((r >> 1) & 1) << 2 | ((r >> 2) & 3));
 }
 
-// Items of 65 to 128 rows (prompts, prefixes that many beams share), head_dim 64 or 128:
+// Groups whose query tiles have 65 to 128 rows (prompts, prefixes that many beams share),
+// head_dim 64 or 128:
 // one workgroup of four waves, 32 rows each, over 64-token tiles, products on
 // v_mfma_f32_32x32x16.  At this many rows an operand is read by every wave, so a tile
 // is turned into 16-bit values once, on its way into LDS: each thread loads its share
@@ -844,7 +845,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_block_kernel(AttnArgs a, int 
   __shared__ int32_t nan_any, k_top;
   // consecutive workgroups are the KV heads of one item: an XCD keeps the same heads in its L2
   const int item = (int)blockIdx.x / a.hkv, kvh = (int)blockIdx.x - item * a.hkv;
-  if (item >= n_items || (a.live_items && item >= *a.live_items)) return;
+  if (item >= (a.live_blocks ? *a.live_blocks : n_items)) return;
 
   const WorkItem it = a.items[item];
   const int tid = threadIdx.x;

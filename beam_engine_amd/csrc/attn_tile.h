@@ -54,6 +54,7 @@ struct AttnArgs {
   const int32_t* merge_rows;
   int32_t* counters;           // [num_merge][hkv] arrivals, zero between runs
   const int32_t* live_items;   // fixed layout: live item count (surplus workgroups exit)
+  const int32_t* live_blocks;  // fixed layout of an 8-bit cache: how many of them are blocks
   int page_size, hkv, hq, g;
   float scale_log2;   // sm_scale * log2(e)
 };

@@ -231,7 +231,8 @@ class BatchedBeamSearch:
         listed = pi.kernel == 4
         caps = dict(max_items=grow * pi.num_items + (64 if listed else 1024), max_queries=n,
                     max_pages=grow * pages + 4096, max_merge=n if listed else n * cfg.num_key_value_heads,
-                    max_merge_rows=grow * pi.num_part_rows + 1024, max_zero=n, tile_rows=64,
+                    max_merge_rows=grow * pi.num_part_rows + 1024, max_zero=n,
+                    tile_rows=128 if listed and pi.num_wg > 0 else 64,
                     max_tails=grow * pi.num_tails + 4096)
         if old is not None:
             caps = {k: max(v, old[k]) for k, v in caps.items()}

@@ -296,8 +296,8 @@ typedef struct be_attn_plan_info {
    * byte-balanced run of (query tile, KV head, 64-token tile) segments;
    * partial results go to per-(query, KV head) slots merged by records.
    * num_items = segments, num_part_rows = slots, num_merge = records.   */
-  int32_t num_wg;          /* persistent workgroups (grid of the attention kernel); kernel 4: items of
-                              more than 64 rows, which come first                  */
+  int32_t num_wg;          /* persistent workgroups (grid of the attention kernel); kernel 4: items on
+                              the block kernel, which come first                   */
   int32_t off_wg;          /* [num_wg][4]: first segment, segments, tiles, 0       */
   int32_t off_records;     /* [grid_merge][8]: query, KV head, first slot entry, slots,
                               first tail entry, tail entries, 0, 0                  */
