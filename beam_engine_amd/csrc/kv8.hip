@@ -11,6 +11,7 @@
 // subnormal step of 2^-24, in fp16.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -21,6 +22,7 @@ constexpr int kLeastExp = -100;        // (2^126 of its inverse stays finite)
 constexpr int kChunk = 16;             // entries of a workgroup, at most
 constexpr int kTile = 256;             // entries of a scan step, members of a batch beyond the chunk's
 constexpr int kMembers = kChunk + kTile;
+constexpr int kHeads = 4;               // KV heads of a pass, at most
 
 // The largest e4m3 value times a power of two that the type holds: stored values
 // saturate there, so that a dequantised value is never an infinity.
@@ -40,6 +42,17 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
 }
 
+// The largest of 16 lanes (a DPP row), in all of them, by rotations of the row.
+template <int N> __device__ __forceinline__ float row_ror(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x120 + N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float max16(float x) {
+  x = fmaxf(x, row_ror<8>(x));
+  x = fmaxf(x, row_ror<4>(x));
+  x = fmaxf(x, row_ror<2>(x));
+  return fmaxf(x, row_ror<1>(x));
+}
+
 struct AppendArgs {
   const void *q, *k, *v;               // rows of head_dim elements, 16-byte aligned; q: with cos only
   int64_t q_sn, k_sn, k_sh, v_sn, v_sh;
@@ -49,17 +62,22 @@ struct AppendArgs {
   uint8_t *kv, *scale;
   const int32_t *page_idx, *slot;
   int32_t* err;
-  int n, hq, hkv, num_pages, page_size, max_pos, chunk;
+  int n, hq, hkv, num_pages, page_size, max_pos;
+  int per_log2;                        // 16-lane groups of an entry: 1 (16 entries a workgroup) or 4 (4 entries)
+  int hq_share, hkv_share;             // heads of a workgroup
 };
 
 // One row of a head over 16 lanes: lane u holds elements u E .. + E - 1 of each half,
 // E = D / 32, in v[0..E) and v[E..2E).
+template <typename T, int E> struct alignas(2 * E) Pack { T x[E]; };
+template <typename T, int E>
+__device__ __forceinline__ void unpack(const Pack<T, E>& p, float (&v)[2 * E], int at) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[at + e] = to_f32(p.x[e]);
+}
 template <typename T, int E>
 __device__ __forceinline__ void load_half(const T* p, float (&v)[2 * E], int at) {
-  struct alignas(2 * E) Pack { T x[E]; };
-  const Pack pk = *reinterpret_cast<const Pack*>(p);
-#pragma unroll
-  for (int e = 0; e < E; ++e) v[at + e] = to_f32(pk.x[e]);
+  unpack<T, E>(*reinterpret_cast<const Pack<T, E>*>(p), v, at);
 }
 
 // HF's rotate_half form in fp32: each product and the sum rounded on its own, so that
@@ -93,17 +111,19 @@ __device__ __forceinline__ void rotate(float (&v)[2 * E], const float (&c)[2 * E
 template <typename T, int D>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   constexpr int E = D / 32;
-  __shared__ int32_t s_page[kChunk], s_lead[kChunk];      // the chunk's pages (-1: not this workgroup's), and which lead
+  __shared__ int32_t s_page[kChunk], s_slot[kChunk], s_lead[kChunk];   // the chunk's pages (-1: skipped), slots, which lead
+  __shared__ bool s_dead[kChunk];                         // written again by a later entry of the chunk
   __shared__ int32_t s_first[kChunk];                     // per led page: least slot written
-  __shared__ uint32_t s_amax[2][kChunk][2];               // per led page, K / V: bits of the largest finite |x|
-  __shared__ int32_t s_exp[kChunk][2], s_old[kChunk][2];  // new and old exponents
+  __shared__ uint32_t s_amax[kHeads][kChunk][2];          // per head, led page, K / V: bits of the largest finite |x|
+  __shared__ int32_t s_exp[kHeads][kChunk][2], s_old[kHeads][kChunk][2];   // new and old exponents
   __shared__ int32_t m_tok[kMembers], m_slot[kMembers];   // a batch: entry, slot, led page, overwritten later
   __shared__ uint8_t m_lead[kMembers], m_dead[kMembers];
   __shared__ int32_t s_range[2], s_wave[4];               // members beyond the chunk: first, last entry; compaction
   __shared__ int32_t s_count, s_grown;
 
   const int tid = threadIdx.x, grp = tid >> 4, u = tid & 15, lane = tid & 63, wave = tid >> 6;
-  const int c0 = blockIdx.x * a.chunk, cn = min(a.chunk, a.n - c0);
+  const int chunk = kChunk >> a.per_log2;
+  const int c0 = blockIdx.x * chunk, cn = min(chunk, a.n - c0);
   const T* cos_t = reinterpret_cast<const T*>(a.cos_t);
   const T* sin_t = reinterpret_cast<const T*>(a.sin_t);
   const bool rope = cos_t != nullptr;
@@ -121,87 +141,172 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     load_half<T, E>(sin_t + p * D + D / 2 + u * E, s, E);
   };
 
-  // ---- the chunk's entries
-  if (tid < kChunk) {
-    int p = -1;
-    if (tid < cn) {
-      if (valid(c0 + tid)) p = a.page_idx[c0 + tid];
-      else if (a.err && blockIdx.y == 0) atomicAdd(a.err, 1);
+  // ---- everything that depends on no other load leaves first: a 16-lane group's entry
+  // (chunk 16: an entry a group; 4: four groups share one's q heads, and its K and V), its
+  // K and V rows of the first heads, its first q rows, and the page ids of the scan
+  const int h0 = blockIdx.y * a.hkv_share, h1 = min(a.hkv, h0 + a.hkv_share);
+  const int per = 1 << a.per_log2, own = grp >> a.per_log2, sub = grp & (per - 1);
+  const bool mine = own < cn;
+  const int64_t tok = c0 + min(own, cn - 1);
+  const int e_page = a.page_idx[tok], e_slot = a.slot[tok];
+  const int64_t e_pos = rope ? a.positions[tok] : 0;
+  constexpr int HB = 8 / E;                            // KV heads of a pass (16 values of a row's 16 lanes each, K and V)
+  Pack<T, E> k_lo[HB], k_hi[HB], v_lo[HB], v_hi[HB];
+  auto load_kv = [&](int h) {
+#pragma unroll
+    for (int b = 0; b < HB; ++b) {
+      if (h + b >= h1) continue;
+      if (per == 1 || sub == 0) {
+        const T* k = reinterpret_cast<const T*>(a.k) + tok * a.k_sn + (int64_t)(h + b) * a.k_sh + u * E;
+        k_lo[b] = *reinterpret_cast<const Pack<T, E>*>(k);
+        k_hi[b] = *reinterpret_cast<const Pack<T, E>*>(k + D / 2);
+      }
+      if (per == 1 || sub == 1) {
+        const T* v = reinterpret_cast<const T*>(a.v) + tok * a.v_sn + (int64_t)(h + b) * a.v_sh + u * E;
+        v_lo[b] = *reinterpret_cast<const Pack<T, E>*>(v);
+        v_hi[b] = *reinterpret_cast<const Pack<T, E>*>(v + D / 2);
+      }
     }
-    s_page[tid] = p;
+  };
+  load_kv(h0);
+  const int q0 = blockIdx.y * a.hq_share, q1 = min(a.hq, q0 + a.hq_share);
+  constexpr int QB = 16 / E;                           // q heads of a pass
+  Pack<T, E> q_lo[QB], q_hi[QB];
+  auto load_q = [&](int h) {
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      if (h + b * per >= q1) continue;
+      const T* src = reinterpret_cast<const T*>(a.q) + tok * a.q_sn + (int64_t)(h + b * per) * D + u * E;
+      q_lo[b] = *reinterpret_cast<const Pack<T, E>*>(src);
+      q_hi[b] = *reinterpret_cast<const Pack<T, E>*>(src + D / 2);
+    }
+  };
+  load_q(q0 + sub);                                    // (hq is 0 without a rotation)
+  constexpr int U = 8;                                 // 16-byte loads of the scan in flight: 8192 entries a round trip
+  const bool vec = (reinterpret_cast<uintptr_t>(a.page_idx) & 15) == 0;
+  int4 ids[U];
+  auto load_ids = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int j = j0 + 1024 * i + 4 * tid;
+      ids[i] = int4{-1, -1, -1, -1};
+      if (vec && j + 3 < a.n) {
+        ids[i] = *reinterpret_cast<const int4*>(a.page_idx + j);
+      } else {
+        if (j < a.n) ids[i].x = a.page_idx[j];
+        if (j + 1 < a.n) ids[i].y = a.page_idx[j + 1];
+        if (j + 2 < a.n) ids[i].z = a.page_idx[j + 2];
+        if (j + 3 < a.n) ids[i].w = a.page_idx[j + 3];
+      }
+    }
+  };
+  load_ids(0);
+
+  // ---- the chunk's entries, the tables of a group's
+  const bool pos_ok = !rope || (e_pos >= 0 && e_pos < a.max_pos);
+  float ct[2 * E], st[2 * E];
+  if (rope && pos_ok) tables(e_pos, ct, st);
+  if (sub == 0 && u == 0) {
+    const bool ok = mine && pos_ok && e_page >= 0 && e_page < a.num_pages && e_slot >= 0 && e_slot < a.page_size;
+    s_page[own] = ok ? e_page : -1;
+    s_slot[own] = e_slot;
+    if (mine && !ok && a.err && blockIdx.y == 0) atomicAdd(a.err, 1);
+  }
+  if (tid < kChunk) {
+    if (tid >= chunk) s_page[tid] = -1;
     s_first[tid] = a.page_size;
   }
   if (tid < 2) s_range[tid] = tid == 0 ? a.n : -1;
-  if (tid < 2 * kChunk) s_amax[0][tid >> 1][tid & 1] = s_amax[1][tid >> 1][tid & 1] = 0;
+  if (tid < kHeads * kChunk * 2) (&s_amax[0][0][0])[tid] = 0;
   __syncthreads();
-  // which entry of the chunk leads its page; a 64-bit filter of the led pages
-  uint64_t filter = 0;
-  for (int i = 0; i < cn; ++i)
-    if (s_page[i] >= 0) filter |= 1ull << (s_page[i] & 63);
-  if (tid < kChunk) {
-    int lead = -1;
-    if (s_page[tid] >= 0) {
-      lead = tid;
-      for (int i = tid - 1; i >= 0; --i)
-        if (s_page[i] == s_page[tid]) lead = i;
+  // which entry of the chunk leads its page, which is written again by a later one of the
+  // chunk (lane i: entry i; every wave for itself); a 64-bit filter of the pages
+  const int w_page = s_page[lane & 15], w_slot = s_slot[lane & 15];
+  int w_lead = -1;
+  bool w_dead = false;
+  uint32_t f0 = 0, f1 = 0;
+#pragma unroll
+  for (int i = kChunk - 1; i >= 0; --i) {
+    const int p = __builtin_amdgcn_readlane(w_page, i), t = __builtin_amdgcn_readlane(w_slot, i);
+    if (p < 0) continue;
+    if (p == w_page) {
+      w_dead = w_dead || (i > (lane & 15) && t == w_slot);
+      w_lead = i;
     }
-    s_lead[tid] = lead;
+    if (p & 32) f1 |= 1u << (p & 31);
+    else f0 |= 1u << (p & 31);
   }
+  if (tid < kChunk) {
+    s_lead[tid] = w_lead;
+    s_dead[tid] = w_dead;
+  }
+  // one or two led pages (prompts): looked for themselves, not by the filter
+  const uint32_t leads = (uint32_t)__ballot(lane < kChunk && w_lead == lane);
+  const int page_a = leads ? __builtin_amdgcn_readlane(w_page, __builtin_ctz(leads)) : -1;
+  const int page_b = leads & (leads - 1) ? __builtin_amdgcn_readlane(w_page, __builtin_ctz(leads & (leads - 1))) : page_a;
+  const bool few = __builtin_popcount(leads) <= 2;
   __syncthreads();
 
   // ---- entries of the led pages outside the chunk
-  {
-    auto look = [&](int j, int p) {
-      if ((uint32_t)p >= (uint32_t)a.num_pages || !((filter >> (p & 63)) & 1)) return;
-      int l = -1;
-      for (int i = 0; i < cn; ++i)
-        if (s_page[i] == p) { l = s_lead[i]; break; }
-      if (l < 0 || (j >= c0 && j < c0 + cn) || !valid(j)) return;
+  auto lead_of = [&](int p) {
+    for (int i = 0; i < cn; ++i)
+      if (s_page[i] == p) return s_lead[i];
+    return -1;
+  };
+  auto maybe = [&](int p) { return ((p & 32 ? f1 : f0) >> (p & 31)) & 1u; };
+  for (int j0 = 0; j0 < a.n; j0 += 1024 * U) {
+    if (j0 > 0) load_ids(j0);
+    uint32_t hits = 0;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (j0 + 1024 * i >= a.n) continue;
+      auto bits = [&](auto test) { return (test(ids[i].x) | test(ids[i].y) << 1 | test(ids[i].z) << 2 | test(ids[i].w) << 3) << (4 * i); };
+      hits |= few ? bits([&](int p) { return (uint32_t)(p == page_a) | (uint32_t)(p == page_b); }) : bits(maybe);
+    }
+    while (hits) {
+      const int bit = __builtin_ctz(hits), j = j0 + 1024 * (bit >> 2) + 4 * tid + (bit & 3);
+      hits &= hits - 1;
+      if (j >= a.n || (j >= c0 && j < c0 + cn)) continue;
+      const int p = a.page_idx[j], l = p >= 0 ? lead_of(p) : -1;
+      if (l < 0 || !valid(j)) continue;
       if (j < c0) {
-        s_first[l] = -1;                             // led by an earlier workgroup
+        s_first[l] = -1;                               // led by an earlier workgroup
       } else {
         atomicMin(&s_range[0], j);
         atomicMax(&s_range[1], j);
       }
-    };
-    // (the least slot is taken below: s_first < 0 marks a page that is not led here)
-    constexpr int U = 8;
-    for (int j0 = tid; j0 < a.n; j0 += 256 * U) {
-      int p[U];
-#pragma unroll
-      for (int i = 0; i < U; ++i) p[i] = j0 + 256 * i < a.n ? a.page_idx[j0 + 256 * i] : -1;
-#pragma unroll
-      for (int i = 0; i < U; ++i) look(j0 + 256 * i, p[i]);
     }
   }
 
-  // ---- q rows of the chunk
-  if (rope && a.hq) {
-    const int h0 = (int)((int64_t)a.hq * blockIdx.y / gridDim.y), h1 = (int)((int64_t)a.hq * (blockIdx.y + 1) / gridDim.y);
-    const int nh = h1 - h0;
-    for (int r = grp; r < cn * nh; r += 16) {
-      const int i = c0 + r / nh, h = h0 + r % nh;
-      const int64_t p = a.positions[i];
-      if (p < 0 || p >= a.max_pos) continue;
-      const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)i * a.q_sn + (int64_t)h * D + u * E;
-      float x[2 * E], c[2 * E], s[2 * E];
-      load_half<T, E>(src, x, 0);
-      load_half<T, E>(src + D / 2, x, E);
-      tables(p, c, s);
-      rotate<E>(x, c, s);
-      struct alignas(2 * E) Pack { T x[E]; } lo, hi;
+  // ---- q rows
+  if (mine && pos_ok) {
+    T* dst = reinterpret_cast<T*>(a.q_out) + tok * a.hq * D + u * E;
+    for (int h = q0 + sub; h < q1; h += QB * per) {
+      Pack<T, E> lo[QB], hi[QB];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        lo.x[e] = from_f32<T>(x[e]);
-        hi.x[e] = from_f32<T>(x[E + e]);
+      for (int b = 0; b < QB; ++b) {
+        lo[b] = q_lo[b];
+        hi[b] = q_hi[b];
       }
-      T* dst = reinterpret_cast<T*>(a.q_out) + ((int64_t)i * a.hq + h) * D + u * E;
-      *reinterpret_cast<Pack*>(dst) = lo;
-      *reinterpret_cast<Pack*>(dst + D / 2) = hi;
+      load_q(h + QB * per);                            // the next pass's, ahead of this one's products
+#pragma unroll
+      for (int b = 0; b < QB; ++b) {
+        if (h + b * per >= q1) continue;
+        float x[2 * E];
+        unpack<T, E>(lo[b], x, 0);
+        unpack<T, E>(hi[b], x, E);
+        rotate<E>(x, ct, st);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          lo[b].x[e] = from_f32<T>(x[e]);
+          hi[b].x[e] = from_f32<T>(x[E + e]);
+        }
+        *reinterpret_cast<Pack<T, E>*>(dst + (h + b * per) * D) = lo[b];
+        *reinterpret_cast<Pack<T, E>*>(dst + (h + b * per) * D + D / 2) = hi[b];
+      }
     }
   }
 
-  const int h0 = (int)((int64_t)a.hkv * blockIdx.y / gridDim.y), h1 = (int)((int64_t)a.hkv * (blockIdx.y + 1) / gridDim.y);
   if (h0 >= h1) return;
   __syncthreads();
 
@@ -216,12 +321,12 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     __syncthreads();
     if (b == 0) {
       if (wave == 0) {
-        const bool mine = lane < cn && s_lead[min(lane, kChunk - 1)] >= 0 && s_first[s_lead[min(lane, kChunk - 1)]] >= 0;
-        const uint64_t bal = __ballot(mine);
-        if (mine) {
+        const bool led = lane < cn && s_lead[min(lane, kChunk - 1)] >= 0 && s_first[s_lead[min(lane, kChunk - 1)]] >= 0;
+        const uint64_t bal = __ballot(led);
+        if (led) {
           const int at = __popcll(bal & ((1ull << lane) - 1));
           m_tok[at] = c0 + lane;
-          m_slot[at] = a.slot[c0 + lane];
+          m_slot[at] = s_slot[lane];
           m_lead[at] = (uint8_t)s_lead[lane];
         }
         if (lane == 0) s_count = __popcll(bal);
@@ -236,9 +341,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       int l = -1;
       if (j < je) {
         const int p = a.page_idx[j];
-        if ((uint32_t)p < (uint32_t)a.num_pages && ((filter >> (p & 63)) & 1) && valid(j)) {
-          for (int i = 0; i < cn; ++i)
-            if (s_page[i] == p) { l = s_lead[i]; break; }
+        if (p >= 0 && maybe(p) && valid(j)) {
+          l = lead_of(p);
           if (l >= 0 && s_first[l] < 0) l = -1;
         }
       }
@@ -275,7 +379,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       rotate<E>(x, c, s);
     }
   };
-  auto take_max = [&](int m, int sel, int buf, const float (&x)[2 * E]) {
+  auto take_max = [&](int lead, int sel, int hi, const float (&x)[2 * E]) {
     float mx = 0.f;
 #pragma unroll
     for (int e = 0; e < 2 * E; ++e) {
@@ -283,14 +387,11 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       mx = fmaxf(mx, y < INFINITY ? y : 0.f);
     }
     mx = fminf(mx, largest<T>());
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 16));
-    if (u == 0) atomicMax(&s_amax[buf][m_lead[m]][sel], __float_as_uint(mx));
+    mx = max16(mx);
+    if (u == 0) atomicMax(&s_amax[hi][lead][sel], __float_as_uint(mx));
   };
-  auto store = [&](int m, int sel, int h, const float (&x)[2 * E]) {
-    if (m_dead[m]) return;
-    const int l = m_lead[m];
-    const float inv = exp2i(-s_exp[l][sel]), top = largest<T>();
+  auto store = [&](int l, int slot, int sel, int h, int hi, const float (&x)[2 * E]) {
+    const float inv = exp2i(-s_exp[hi][l][sel]), top = largest<T>();
     float y[2 * E];
 #pragma unroll
     for (int e = 0; e < 2 * E; ++e) {
@@ -298,7 +399,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       const float z = fabsf(x[e]) < INFINITY ? fminf(fmaxf(x[e], -top), top) : x[e];
       y[e] = z * inv;
     }
-    uint8_t* dst = a.kv + ((((int64_t)s_page[l] * 2 + sel) * a.page_size + m_slot[m]) * a.hkv + h) * D + u * E;
+    uint8_t* dst = a.kv + ((((int64_t)s_page[l] * 2 + sel) * a.page_size + slot) * a.hkv + h) * D + u * E;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int o = half * E;
@@ -314,6 +415,99 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     }
   };
 
+  // the old exponents of a pass's blocks, ahead of what they are compared with: thread
+  // (head, page, K / V)
+  auto scale_at = [&](int h) { return a.scale + ((int64_t)s_page[(tid >> 1) & 15] * 2 + (tid & 1)) * a.hkv + h; };
+  auto is_block = [&](int l) { return s_lead[l] == l && s_first[l] >= 0 && s_first[l] < a.page_size; };
+  auto old_exp = [&](int h, int nh) {
+    const int l = (tid >> 1) & 15, hi = tid >> 5;
+    return hi < nh && is_block(l) && s_first[l] > 0 ? min((int)*scale_at(h + hi) - 127, 120) : 0;   // (120: a bf16 block's most)
+  };
+  auto new_exp = [&](int h, int nh, int old) {
+    const int l = (tid >> 1) & 15, sel = tid & 1, hi = tid >> 5;
+    if (hi >= nh) return;
+    int e = 0;
+    if (is_block(l)) {
+      e = block_exp(s_amax[hi][l][sel]);
+      if (s_first[l] > 0) {
+        e = max(e, old);
+        if (e > old) s_grown = 1;
+      } else {
+        old = e;
+      }
+      *scale_at(h + hi) = (uint8_t)(e + 127);
+    } else {
+      old = 0;
+    }
+    s_exp[hi][l][sel] = e;
+    s_old[hi][l][sel] = old;
+    s_amax[hi][l][sel] = 0;
+  };
+  // tokens written before, where a scale grew
+  auto rescale = [&](int h, int nh) {
+    for (int hi = 0; hi < nh; ++hi)
+      for (int l = 0; l < cn; ++l)
+        for (int sel = 0; sel < 2; ++sel) {
+          const int by = s_old[hi][l][sel] - s_exp[hi][l][sel];
+          if (by >= 0) continue;
+          const float f = exp2i(max(by, -126));
+          for (int t = grp; t < s_first[l]; t += 16) {
+            uint8_t* d = a.kv + ((((int64_t)s_page[l] * 2 + sel) * a.page_size + t) * a.hkv + h + hi) * D + u * (D / 16);
+#pragma unroll
+            for (int w = 0; w < D / 64; ++w) {
+              typedef float f2 __attribute__((ext_vector_type(2)));
+              const int c = *reinterpret_cast<const int*>(d + 4 * w);
+              const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), hi2 = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+              *reinterpret_cast<uint32_t*>(d + 4 * w) = codes4(lo.x * f, lo.y * f, hi2.x * f, hi2.y * f);
+            }
+          }
+        }
+  };
+
+  // ---- no entry outside the chunk belongs to its pages (a decode step, prompts that start
+  // at a chunk): the groups' own rows, which are there already
+  if (tiles == 0) {
+    const int l = s_lead[own];
+    const bool led = mine && l >= 0 && s_first[max(l, 0)] >= 0;
+    __syncthreads();
+    if (led && sub == 0 && u == 0) atomicMin(&s_first[l], e_slot);
+    __syncthreads();
+    const bool write = led && !s_dead[own];
+    for (int h = h0; h < h1; h += HB) {
+      const int nh = min(HB, h1 - h), old = old_exp(h, nh);
+      if (h > h0) load_kv(h);
+      float xk[HB][2 * E], xv[HB][2 * E];
+#pragma unroll
+      for (int b = 0; b < HB; ++b) {
+        if (!led || b >= nh) continue;
+        if (per == 1 || sub == 0) {
+          unpack<T, E>(k_lo[b], xk[b], 0);
+          unpack<T, E>(k_hi[b], xk[b], E);
+          if (rope) rotate<E>(xk[b], ct, st);
+          take_max(l, 0, b, xk[b]);
+        }
+        if (per == 1 || sub == 1) {
+          unpack<T, E>(v_lo[b], xv[b], 0);
+          unpack<T, E>(v_hi[b], xv[b], E);
+          take_max(l, 1, b, xv[b]);
+        }
+      }
+      if (tid == 0) s_grown = 0;
+      __syncthreads();
+      new_exp(h, nh, old);
+      __syncthreads();
+#pragma unroll
+      for (int b = 0; b < HB; ++b) {
+        if (!write || b >= nh) continue;
+        if (per == 1 || sub == 0) store(l, e_slot, 0, h + b, b, xk[b]);
+        if (per == 1 || sub == 1) store(l, e_slot, 1, h + b, b, xv[b]);
+      }
+      if (s_grown) rescale(h, nh);
+      __syncthreads();
+    }
+    return;
+  }
+
   collect(0);
   const bool single = tiles <= 1;
   if (single && members == 0) return;
@@ -322,89 +516,82 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     collect(b);
     for (int m = tid; m < members; m += 256) atomicMin(&s_first[m_lead[m]], m_slot[m]);
   }
-  const bool cached = single && 2 * members <= 32;     // at most two rows a 16-lane group, kept in registers
-
-  for (int h = h0; h < h1; ++h) {
-    const int buf = h & 1;
-    float keep[2][2 * E];
-    if (cached) {
+  __syncthreads();                                   // the least slots are known
+  // a few members: a head's rows in registers, one or two a group
+  auto held = [&](auto mp_) {
+    constexpr int MP = decltype(mp_)::value;
+    float c[MP][2 * E], s[MP][2 * E];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = grp + 16 * i;
-        if (r < 2 * members) {
-          row(m_tok[r >> 1], r & 1, h, keep[i]);
-          take_max(r >> 1, r & 1, buf, keep[i]);
-        }
+    for (int m = 0; m < MP; ++m)
+      if (rope && grp + 16 * m < members) tables(a.positions[m_tok[grp + 16 * m]], c[m], s[m]);
+    for (int h = h0; h < h1; ++h) {
+      const int old = old_exp(h, 1);
+      float x[MP][2][2 * E];
+#pragma unroll
+      for (int m = 0; m < MP; ++m) {
+        if (grp + 16 * m >= members) continue;
+        const int64_t t = m_tok[grp + 16 * m];
+        const T* k = reinterpret_cast<const T*>(a.k) + t * a.k_sn + (int64_t)h * a.k_sh + u * E;
+        const T* v = reinterpret_cast<const T*>(a.v) + t * a.v_sn + (int64_t)h * a.v_sh + u * E;
+        load_half<T, E>(k, x[m][0], 0);
+        load_half<T, E>(k + D / 2, x[m][0], E);
+        load_half<T, E>(v, x[m][1], 0);
+        load_half<T, E>(v + D / 2, x[m][1], E);
       }
-    } else {
+#pragma unroll
+      for (int m = 0; m < MP; ++m) {
+        if (grp + 16 * m >= members) continue;
+        if (rope) rotate<E>(x[m][0], c[m], s[m]);
+        take_max(m_lead[grp + 16 * m], 0, 0, x[m][0]);
+        take_max(m_lead[grp + 16 * m], 1, 0, x[m][1]);
+      }
+      if (tid == 0) s_grown = 0;
+      __syncthreads();
+      new_exp(h, 1, old);
+      __syncthreads();
+#pragma unroll
+      for (int m = 0; m < MP; ++m) {
+        const int i = grp + 16 * m;
+        if (i >= members || m_dead[i]) continue;
+        store(m_lead[i], m_slot[i], 0, h, 0, x[m][0]);
+        store(m_lead[i], m_slot[i], 1, h, 0, x[m][1]);
+      }
+      if (s_grown) rescale(h, 1);
+      __syncthreads();
+    }
+  };
+  if (single && members <= 16) {
+    held(std::integral_constant<int, 1>());
+  } else if (single && members <= 32) {
+    held(std::integral_constant<int, 2>());
+  } else {
+    for (int h = h0; h < h1; ++h) {
+      const int old = old_exp(h, 1);
       for (int b = 0; b <= (single ? 0 : tiles); ++b) {
         if (!single) collect(b);
         for (int r = grp; r < 2 * members; r += 16) {
           float x[2 * E];
           row(m_tok[r >> 1], r & 1, h, x);
-          take_max(r >> 1, r & 1, buf, x);
+          take_max(m_lead[r >> 1], r & 1, 0, x);
         }
       }
-    }
-    if (tid == 0) s_grown = 0;
-    __syncthreads();
-    // ---- the blocks' new scales
-    if (tid < 2 * kChunk) {
-      const int l = tid >> 1, sel = tid & 1;
-      s_amax[buf ^ 1][l][sel] = 0;
-      if (s_lead[l] == l && s_first[l] >= 0 && s_first[l] < a.page_size) {
-        uint8_t* sp = a.scale + ((int64_t)s_page[l] * 2 + sel) * a.hkv + h;
-        int e = block_exp(s_amax[buf][l][sel]), old = e;
-        if (s_first[l] > 0) {
-          old = min((int)*sp - 127, 120);            // (120: the largest of a bf16 block)
-          e = max(e, old);
-          if (e > old) s_grown = 1;
-        }
-        s_exp[l][sel] = e;
-        s_old[l][sel] = old;
-        *sp = (uint8_t)(e + 127);
-      } else {
-        s_exp[l][sel] = s_old[l][sel] = 0;
-      }
-    }
-    __syncthreads();
-    // ---- the members' codes
-    if (cached) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = grp + 16 * i;
-        if (r < 2 * members) store(r >> 1, r & 1, h, keep[i]);
-      }
-    } else {
+      if (tid == 0) s_grown = 0;
+      __syncthreads();
+      new_exp(h, 1, old);
+      __syncthreads();
       for (int b = 0; b <= (single ? 0 : tiles); ++b) {
         if (!single) collect(b);
         for (int r = grp; r < 2 * members; r += 16) {
+          const int m = r >> 1;
+          if (m_dead[m]) continue;
           float x[2 * E];
-          row(m_tok[r >> 1], r & 1, h, x);
-          store(r >> 1, r & 1, h, x);
+          row(m_tok[m], r & 1, h, x);
+          store(m_lead[m], m_slot[m], r & 1, h, 0, x);
         }
       }
+      if (s_grown) rescale(h, 1);
+      __syncthreads();
     }
-    // ---- tokens written before, where the scale grew
-    if (s_grown) {
-      for (int l = 0; l < cn; ++l)
-        for (int sel = 0; sel < 2; ++sel) {
-          const int by = s_old[l][sel] - s_exp[l][sel];
-          if (by >= 0) continue;
-          const float f = exp2i(max(by, -126));
-          for (int t = grp; t < s_first[l]; t += 16) {
-            uint8_t* d = a.kv + ((((int64_t)s_page[l] * 2 + sel) * a.page_size + t) * a.hkv + h) * D + u * (D / 16);
-#pragma unroll
-            for (int w = 0; w < D / 64; ++w) {
-              typedef float f2 __attribute__((ext_vector_type(2)));
-              const int c = *reinterpret_cast<const int*>(d + 4 * w);
-              const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
-              *reinterpret_cast<uint32_t*>(d + 4 * w) = codes4(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
-            }
-          }
-        }
-    }
-    __syncthreads();
   }
 }
 
@@ -481,12 +668,15 @@ static int check_cache(const void* kv, const void* scale, int num_pages, int pag
 
 // Entries of a workgroup and its share of the heads.  Few entries: four a workgroup
 // and one KV head each, so that a decode step's rows spread over the CUs; many: 16 (a
-// page's worth), and just enough shares to give every CU a few workgroups.
+// page's worth), and as few shares as leave every CU four workgroups.
 static int launch_append(AppendArgs& a, int dtype, int d, hipStream_t st) {
-  a.chunk = a.n <= 1024 ? 4 : kChunk;
-  const unsigned gx = (unsigned)((a.n + a.chunk - 1) / a.chunk);
-  const unsigned gy = (unsigned)std::min<int64_t>(a.hkv, std::max<int64_t>(1, (2048 + gx - 1) / gx));
-  const dim3 grid(gx, gy);
+  a.per_log2 = a.n <= 1024 ? 2 : 0;
+  const int chunk = kChunk >> a.per_log2;
+  const unsigned gx = (unsigned)((a.n + chunk - 1) / chunk);
+  const int shares = (int)std::min<int64_t>(a.hkv, std::max<int64_t>(1, (1024 + gx - 1) / gx));
+  a.hkv_share = (a.hkv + shares - 1) / shares;
+  a.hq_share = (a.hq + shares - 1) / shares;
+  const dim3 grid(gx, (unsigned)shares);
 #define BE_APPEND(TY)                                                        \
   switch (d) {                                                               \
     case 64: append_kernel<TY, 64><<<grid, 256, 0, st>>>(a); break;          \
