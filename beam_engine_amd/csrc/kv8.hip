@@ -63,7 +63,6 @@ struct AppendArgs {
   const int32_t *page_idx, *slot;
   int32_t* err;
   int n, hq, hkv, num_pages, page_size, max_pos;
-  int per_log2;                        // 16-lane groups of an entry: 1 (16 entries a workgroup) or 4 (4 entries)
   int hq_share, hkv_share;             // heads of a workgroup
 };
 
@@ -108,7 +107,7 @@ __device__ __forceinline__ void rotate(float (&v)[2 * E], const float (&c)[2 * E
 //
 // What bounds it: a decode step's launch is a chain of round trips (indices, rows,
 // tables, the old scale); prompts are bound by the rows' bytes.
-template <typename T, int D>
+template <typename T, int D, int PER>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   constexpr int E = D / 32;
   __shared__ int32_t s_page[kChunk], s_slot[kChunk], s_lead[kChunk];   // the chunk's pages (-1: skipped), slots, which lead
@@ -122,7 +121,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   __shared__ int32_t s_count, s_grown;
 
   const int tid = threadIdx.x, grp = tid >> 4, u = tid & 15, lane = tid & 63, wave = tid >> 6;
-  const int chunk = kChunk >> a.per_log2;
+  constexpr int chunk = kChunk / PER, per = PER;       // entries, and 16-lane groups of one
   const int c0 = blockIdx.x * chunk, cn = min(chunk, a.n - c0);
   const T* cos_t = reinterpret_cast<const T*>(a.cos_t);
   const T* sin_t = reinterpret_cast<const T*>(a.sin_t);
@@ -145,7 +144,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   // (chunk 16: an entry a group; 4: four groups share one's q heads, and its K and V), its
   // K and V rows of the first heads, its first q rows, and the page ids of the scan
   const int h0 = blockIdx.y * a.hkv_share, h1 = min(a.hkv, h0 + a.hkv_share);
-  const int per = 1 << a.per_log2, own = grp >> a.per_log2, sub = grp & (per - 1);
+  const int own = grp / per, sub = grp % per;
   const bool mine = own < cn;
   const int64_t tok = c0 + min(own, cn - 1);
   const int e_page = a.page_idx[tok], e_slot = a.slot[tok];
@@ -182,23 +181,11 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     }
   };
   load_q(q0 + sub);                                    // (hq is 0 without a rotation)
-  constexpr int U = 8;                                 // 16-byte loads of the scan in flight: 8192 entries a round trip
-  const bool vec = (reinterpret_cast<uintptr_t>(a.page_idx) & 15) == 0;
-  int4 ids[U];
+  constexpr int U = PER == 1 ? 8 : 4;                  // ids of a thread in flight (4: all of 1024 entries)
+  int ids[U];
   auto load_ids = [&](int j0) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int j = j0 + 1024 * i + 4 * tid;
-      ids[i] = int4{-1, -1, -1, -1};
-      if (vec && j + 3 < a.n) {
-        ids[i] = *reinterpret_cast<const int4*>(a.page_idx + j);
-      } else {
-        if (j < a.n) ids[i].x = a.page_idx[j];
-        if (j + 1 < a.n) ids[i].y = a.page_idx[j + 1];
-        if (j + 2 < a.n) ids[i].z = a.page_idx[j + 2];
-        if (j + 3 < a.n) ids[i].w = a.page_idx[j + 3];
-      }
-    }
+    for (int i = 0; i < U; ++i) ids[i] = j0 + 256 * i + tid < a.n ? a.page_idx[j0 + 256 * i + tid] : -1;
   };
   load_ids(0);
 
@@ -254,17 +241,13 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     return -1;
   };
   auto maybe = [&](int p) { return ((p & 32 ? f1 : f0) >> (p & 31)) & 1u; };
-  for (int j0 = 0; j0 < a.n; j0 += 1024 * U) {
-    if (j0 > 0) load_ids(j0);
+  for (int j0 = 0; j0 < a.n; j0 += 256 * U) {
     uint32_t hits = 0;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (j0 + 1024 * i >= a.n) continue;
-      auto bits = [&](auto test) { return (test(ids[i].x) | test(ids[i].y) << 1 | test(ids[i].z) << 2 | test(ids[i].w) << 3) << (4 * i); };
-      hits |= few ? bits([&](int p) { return (uint32_t)(p == page_a) | (uint32_t)(p == page_b); }) : bits(maybe);
-    }
+    for (int i = 0; i < U; ++i) hits |= (few ? (uint32_t)(ids[i] == page_a) | (uint32_t)(ids[i] == page_b) : maybe(ids[i])) << i;
+    if (PER == 1) load_ids(j0 + 256 * U);              // the next ones', ahead of these ones' hits
     while (hits) {
-      const int bit = __builtin_ctz(hits), j = j0 + 1024 * (bit >> 2) + 4 * tid + (bit & 3);
+      const int j = j0 + 256 * __builtin_ctz(hits) + tid;
       hits &= hits - 1;
       if (j >= a.n || (j >= c0 && j < c0 + cn)) continue;
       const int p = a.page_idx[j], l = p >= 0 ? lead_of(p) : -1;
@@ -666,22 +649,27 @@ static int check_cache(const void* kv, const void* scale, int num_pages, int pag
   return BE_OK;
 }
 
-// Entries of a workgroup and its share of the heads.  Few entries: four a workgroup
-// and one KV head each, so that a decode step's rows spread over the CUs; many: 16 (a
-// page's worth), and as few shares as leave every CU four workgroups.
+// Few entries (a decode step): four a workgroup and one KV head each, so that their rows
+// spread over the CUs; many: 16 (a page's worth), and as few shares of the heads as leave
+// every CU four workgroups.
+constexpr int kFew = 1024;
+template <typename T, int D>
+static void launch_per(const AppendArgs& a, dim3 grid, hipStream_t st) {
+  if (a.n <= kFew) append_kernel<T, D, 4><<<grid, 256, 0, st>>>(a);
+  else append_kernel<T, D, 1><<<grid, 256, 0, st>>>(a);
+}
 static int launch_append(AppendArgs& a, int dtype, int d, hipStream_t st) {
-  a.per_log2 = a.n <= 1024 ? 2 : 0;
-  const int chunk = kChunk >> a.per_log2;
+  const int chunk = a.n <= kFew ? kChunk / 4 : kChunk;
   const unsigned gx = (unsigned)((a.n + chunk - 1) / chunk);
   const int shares = (int)std::min<int64_t>(a.hkv, std::max<int64_t>(1, (1024 + gx - 1) / gx));
   a.hkv_share = (a.hkv + shares - 1) / shares;
   a.hq_share = (a.hq + shares - 1) / shares;
   const dim3 grid(gx, (unsigned)shares);
-#define BE_APPEND(TY)                                                        \
-  switch (d) {                                                               \
-    case 64: append_kernel<TY, 64><<<grid, 256, 0, st>>>(a); break;          \
-    case 128: append_kernel<TY, 128><<<grid, 256, 0, st>>>(a); break;        \
-    default: append_kernel<TY, 256><<<grid, 256, 0, st>>>(a); break;         \
+#define BE_APPEND(TY)                                       \
+  switch (d) {                                              \
+    case 64: launch_per<TY, 64>(a, grid, st); break;        \
+    case 128: launch_per<TY, 128>(a, grid, st); break;      \
+    default: launch_per<TY, 256>(a, grid, st); break;       \
   }
   if (dtype == BE_BF16) { BE_APPEND(bf16_t) } else { BE_APPEND(f16_t) }
 #undef BE_APPEND
