@@ -343,14 +343,15 @@ class _PagedPlanner:
         if kv8:
             args = (ctypes.byref(info), self._plan_dev.data_ptr(), _lib.ptr(self._partials), qp, sn, sh, kv.data_ptr(),
                     kv_scale.data_ptr(), op, on, oh, _lib.ptr(lse), self._sm_scale)
-            with _lib.on_device(q):
-                if between is None:
-                    _lib.check(lib.be_attn_run_kv8(*args, _lib.BE_RUN_ATTENTION | _lib.BE_RUN_MERGE, stream),
-                               "attention run")
-                else:
-                    _lib.check(lib.be_attn_run_kv8(*args, _lib.BE_RUN_ATTENTION, stream), "attention run")
-                    between()
-                    _lib.check(lib.be_attn_run_kv8(*args, _lib.BE_RUN_MERGE, stream), "attention merge")
+            if torch._C._cuda_getDevice() != dev:
+                with torch.cuda.device(dev):
+                    self._run_kv8(lib, args, stream, between)
+            elif between is None:
+                rc = lib.be_attn_run_kv8(*args, _lib.BE_RUN_ATTENTION | _lib.BE_RUN_MERGE, stream)
+                if rc:
+                    _lib.check(rc, "attention run")
+            else:
+                self._run_kv8(lib, args, stream, between)
             return (out, lse) if return_lse else out
         args = (ctypes.byref(info), self._plan_dev.data_ptr(), _lib.ptr(self._partials), qp, sn, sh, kv.data_ptr(), op,
                 on, oh, _lib.ptr(lse), self._sm_scale)
@@ -363,6 +364,15 @@ class _PagedPlanner:
             between()
             _lib.check(lib.be_attn_run(*args, _lib.BE_RUN_MERGE, stream), "attention merge")
         return (out, lse) if return_lse else out
+
+    @staticmethod
+    def _run_kv8(lib, args, stream: int, between) -> None:
+        if between is None:
+            _lib.check(lib.be_attn_run_kv8(*args, _lib.BE_RUN_ATTENTION | _lib.BE_RUN_MERGE, stream), "attention run")
+            return
+        _lib.check(lib.be_attn_run_kv8(*args, _lib.BE_RUN_ATTENTION, stream), "attention run")
+        between()
+        _lib.check(lib.be_attn_run_kv8(*args, _lib.BE_RUN_MERGE, stream), "attention merge")
 
     def use_fixed_layout(self, max_items: int, max_queries: int, max_pages: int, max_merge: int,
                          max_merge_rows: int, max_zero: int, tile_rows: int, max_tails: int = 0) -> None:

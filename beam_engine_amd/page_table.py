@@ -115,6 +115,11 @@ class PageTable:
         self._err = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._err_host = torch.zeros(1, dtype=torch.int32, pin_memory=self.device.type == "cuda")
         self._err_np = self._err_host.numpy()     # its numpy view (a cheap read after each synchronisation)
+        if self.kv8:                              # addresses of a launch, kept
+            self._dev_index = self.kv_pool.get_device()
+            self._dtype_code = _lib.dtype_code(self.compute_dtype)
+            self._kv_ptr, self._scale_ptr = self.kv_pool.data_ptr(), self.kv_scale.data_ptr()
+            self._scale_stride, self._err_ptr = self.kv_scale.stride(0), self._err.data_ptr()
         logger.info("Initialized PageTable: %d layers, %d pages of size %d", layer_num, max_num_pages, page_size)
 
     # ------------------------------------------------------------ allocator
@@ -458,13 +463,14 @@ class PageTable:
         tensor code does."""
         if layer < 0 or layer >= self.layer_num:
             raise ValueError(f"Layer {layer} out of range (max: {self.layer_num - 1})")
+        if self.kv8:
+            return self._rope_kv8(layer, qkv, num_qo_heads, positions, cos, sin, page_indices, indices, q_out)
         n = qkv.shape[0]
         width = (num_qo_heads + 2 * self.head_num) * self.head_dim
         if qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
             raise ValueError(f"qkv must be [N, {width}] with a contiguous last dim")
-        dt = self.compute_dtype
-        if qkv.dtype != dt or cos.dtype != dt or sin.dtype != dt:
-            raise ValueError(f"qkv and cos/sin tables must be {dt}")
+        if qkv.dtype != self.store_dtype or cos.dtype != self.store_dtype or sin.dtype != self.store_dtype:
+            raise ValueError(f"qkv and cos/sin tables must be {self.store_dtype}")
         if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != self.head_dim or not cos.is_contiguous() \
                 or not sin.is_contiguous():
             raise ValueError("cos/sin must be contiguous [max_pos, head_dim]")
@@ -478,8 +484,6 @@ class PageTable:
             q_out = torch.empty((n, num_qo_heads, self.head_dim), dtype=qkv.dtype, device=qkv.device)
         elif q_out.shape != (n, num_qo_heads, self.head_dim) or not q_out.is_contiguous() or q_out.dtype != qkv.dtype:
             raise ValueError("q_out must be a contiguous [N, Hq, D] tensor of the storage dtype")
-        if self.kv8:
-            return self._rope_kv8(layer, qkv, num_qo_heads, positions, cos, sin, page_indices, indices, q_out, n)
         lib = _lib.load()
         rc = lib.be_rope_qkv_append(qkv.data_ptr(), qkv.stride(0), _lib.dtype_code(self.store_dtype), n, num_qo_heads,
                                     self.head_num, self.head_dim, positions.data_ptr(), cos.data_ptr(),
@@ -491,24 +495,49 @@ class PageTable:
         return q_out
 
     def _rope_kv8(self, layer: int, qkv: torch.Tensor, hq: int, positions: torch.Tensor, cos: torch.Tensor,
-                  sin: torch.Tensor, pages: torch.Tensor, slots: torch.Tensor, q_out: torch.Tensor, n: int) -> torch.Tensor:
-        self._same_device((qkv, "qkv"), (positions, "positions"), (cos, "cos"), (sin, "sin"), (pages, "page_indices"),
-                          (slots, "indices"), (q_out, "q_out"))
-        positions, pages, slots = (t if t.is_contiguous() else t.reshape(-1).contiguous() for t in (positions, pages, slots))
-        if qkv.data_ptr() % 16 or qkv.stride(0) % 8:
-            qkv = qkv.clone(memory_format=torch.contiguous_format)
-        cos, sin = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (cos, sin))
-        if n and q_out.data_ptr() % 16:
-            raise ValueError("q_out must be 16-byte aligned")
-        with _lib.on_device(self.kv_pool):
-            rc = self._lib.be_kv8_rope_append(qkv.data_ptr(), qkv.stride(0), _lib.dtype_code(self.compute_dtype), n, hq,
-                                              self.head_num, self.head_dim, positions.data_ptr(), cos.data_ptr(),
-                                              sin.data_ptr(), cos.shape[0], q_out.data_ptr(),
-                                              self.kv_cache_at_layer[layer].data_ptr(),
-                                              self.kv_scale_at_layer[layer].data_ptr(), self.max_num_pages, self.page_size,
-                                              pages.data_ptr(), slots.data_ptr(), self._err.data_ptr(),
-                                              _lib.stream_ptr(self.device))
-        _lib.check(rc, "rope append")
+                  sin: torch.Tensor, pages: torch.Tensor, slots: torch.Tensor, q_out: Optional[torch.Tensor]) -> torch.Tensor:
+        # (a decode step's launch takes 8 us on the GPU, so this call's own time shows:
+        # every property is read once, and the cache's addresses are kept)
+        n, d, dt, dev = qkv.shape[0], self.head_dim, self.compute_dtype, self._dev_index
+        if qkv.dtype is not dt or cos.dtype is not dt or sin.dtype is not dt:
+            raise ValueError(f"qkv and cos/sin tables must be {dt}")
+        if qkv.get_device() != dev or positions.get_device() != dev or cos.get_device() != dev or sin.get_device() != dev or \
+                pages.get_device() != dev or slots.get_device() != dev or dev < 0:
+            for t, nm in ((qkv, "qkv"), (positions, "positions"), (pages, "page_indices"), (slots, "indices")):
+                _lib.require_device(t, nm)
+            raise ValueError(f"qkv, positions, tables, page_indices and indices must be on the cache's device {self.device}")
+        width = (hq + 2 * self.head_num) * d
+        sn, sd = qkv.stride() if qkv.dim() == 2 else (0, 0)
+        if qkv.dim() != 2 or qkv.shape[1] != width or sd != 1 or hq < 1:
+            raise ValueError(f"qkv must be [N, {width}] with a contiguous last dim")
+        if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != d or not cos.is_contiguous() or not sin.is_contiguous():
+            raise ValueError("cos/sin must be contiguous [max_pos, head_dim]")
+        if positions.dtype is not torch.int64 or pages.dtype is not torch.int32 or slots.dtype is not torch.int32:
+            raise ValueError("positions must be int64, page_indices / indices int32")
+        if positions.numel() < n or pages.numel() < n or slots.numel() < n:
+            raise ValueError("positions / page_indices / indices shorter than qkv")
+        if q_out is None:
+            q_out = torch.empty((n, hq, d), dtype=dt, device=qkv.device)
+        elif q_out.shape != (n, hq, d) or not q_out.is_contiguous() or q_out.dtype is not dt or q_out.get_device() != dev or \
+                (n and q_out.data_ptr() % 16):
+            raise ValueError("q_out must be a contiguous, 16-byte aligned [N, Hq, D] tensor of the compute dtype on the cache's "
+                             "device")
+        if not (positions.is_contiguous() and pages.is_contiguous() and slots.is_contiguous()):
+            positions, pages, slots = (t.reshape(-1).contiguous() for t in (positions, pages, slots))
+        x, c, s = qkv.data_ptr(), cos.data_ptr(), sin.data_ptr()
+        if (x | c | s) % 16 or sn % 8:
+            qkv, cos, sin = (t.clone(memory_format=torch.contiguous_format) for t in (qkv, cos, sin))
+            x, c, s, sn = qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), width
+        args = (x, sn, self._dtype_code, n, hq, self.head_num, d, positions.data_ptr(), c, s, cos.shape[0], q_out.data_ptr(),
+                self._kv_ptr + layer * self.layer_stride_bytes, self._scale_ptr + layer * self._scale_stride,
+                self.max_num_pages, self.page_size, pages.data_ptr(), slots.data_ptr(), self._err_ptr, _lib.raw_stream(qkv))
+        if torch._C._cuda_getDevice() == dev:
+            rc = self._lib.be_kv8_rope_append(*args)
+        else:
+            with torch.cuda.device(dev):
+                rc = self._lib.be_kv8_rope_append(*args)
+        if rc:
+            _lib.check(rc, "rope append")
         return q_out
 
     # ------------------------------------------------------------ flat views
