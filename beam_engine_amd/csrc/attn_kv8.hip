@@ -985,14 +985,18 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_block_kernel(AttnArgs a, int 
   for (int tile = 0; tile < n_tiles; ++tile) {
     const int st = tile & 1;
     stream::lds_sync();                              // the tile is in its stage, and everyone is done with the other
+    const int t0 = tile * kTile;
+    const unsigned char* kt = stage + st * STAGE;
+    const unsigned char* vt = kt + PLANE;
+    // the first K fragments leave LDS while the next tile is converted
+    v8s kf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const v8s*>(kt + koff[ks]);
     if (tile + 1 < n_tiles) {
       put(tile + 1, stage + (st ^ 1) * STAGE);
       if (tile + 2 < n_tiles) fetch(tile + 2);
     }
-    const int t0 = tile * kTile;
     if (!wave_on || t0 >= lim_most) continue;
-    const unsigned char* kt = stage + st * STAGE;
-    const unsigned char* vt = kt + PLANE;
 
     v16f x[2];
 #pragma unroll
@@ -1000,13 +1004,11 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_block_kernel(AttnArgs a, int 
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[tb][i] = 0.f;
 #pragma unroll
-    for (int tb = 0; tb < 2; ++tb) {
-      v8s kf[KS];
+    for (int ks = 0; ks < KS; ++ks) x[0] = mfma32<T>(kf[ks], qf[ks], x[0]);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const v8s*>(kt + tb * 32 * RB + koff[ks]);
+    for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const v8s*>(kt + 32 * RB + koff[ks]);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) x[tb] = mfma32<T>(kf[ks], qf[ks], x[tb]);
-    }
+    for (int ks = 0; ks < KS; ++ks) x[1] = mfma32<T>(kf[ks], qf[ks], x[1]);
     if (__builtin_amdgcn_ballot_w64(lim < t0 + kTile) != 0) {
       const int left = lim - t0 - 4 * h;
 #pragma unroll
