@@ -635,14 +635,20 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   if (any_causal)
     std::stable_sort(items.begin(), items.end(), [](const WorkItem& x, const WorkItem& y) { return x.tok_count > y.tok_count; });
 
-  // an 8-bit cache: items of more than 64 rows first, which the block kernel takes
-  int block_items = 0;
+  // an 8-bit cache: the block kernel's items first, those of one wave each last
+  int block_items = 0, wave_items = 0;
   if (kv8) {
     // (a block's last, smaller query tiles go with it: alone they would be a launch of a few
     // long chains behind it)
     const auto rest = std::stable_partition(items.begin(), items.end(), [](const WorkItem& w) { return w.first_page < 0; });
     block_items = (int)(rest - items.begin());
     for (int i = 0; i < block_items; ++i) items[i].first_page = ~items[i].first_page;
+    if (page_size % 16 == 0) {
+      const auto waves = std::stable_partition(rest, items.end(), [&](const WorkItem& w) {
+        return w.q_count * g > 16 || w.tok_count > kWaveTokens || w.vis0 != kNoCausal;
+      });
+      wave_items = (int)(items.end() - waves);
+    }
   }
 
   // ---- merge list (queries with partial rows: one of a tile whose other queries
@@ -693,7 +699,10 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   out[kHdrMerge] = (int32_t)merge_q.size();
   out[kHdrZero] = (int32_t)zero_q.size();
   out[kHdrRows] = rows;
-  if (kv8) out[kHdrBlocks] = block_items;
+  if (kv8) {
+    out[kHdrBlocks] = block_items;
+    out[kHdrWaves] = wave_items;
+  }
   memcpy(out + off_items, items.data(), n_items * sizeof(WorkItem));
   for (int i = 0; i < num_queries; ++i) out[off_qindex + i] = i;
   {
@@ -726,6 +735,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   info->dtype = dtype;
   info->kernel = kv8 ? 4 : blocks ? 2 : mfma ? 1 : 0;
   info->stream_loop = blocks ? kLoopBlocks : 0;
+  info->num_tail_items = wave_items;
   info->num_wg = !kv8 ? 0 : caps && rows_cap > 64 ? (int)c_items : block_items;
   info->tile_rows = !mfma && !f32 ? 0 : blocks ? 128 : caps ? (f32 || kv8 ? rows_cap : caps->tile_rows) : (max_r <= 16 ? 16 : max_r <= 32 ? 32 : max_r <= 64 ? 64 : 128);
   info->chunk_tokens = (int32_t)std::min<int64_t>(kv8_chunk > 0 ? std::min(kv8_chunk, chunk_cap) : causal_chunk > 0 ? std::min(causal_chunk, chunk_cap) : chunk, INT32_MAX);

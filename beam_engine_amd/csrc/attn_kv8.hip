@@ -263,6 +263,13 @@ struct Codes {
   }
 };
 
+// An item's record by scalar loads, whatever the compiler can tell of its index.
+__device__ __forceinline__ WorkItem item_at(const AttnArgs& a, int i) {
+  typedef const int32_t __attribute__((address_space(4)))* words_t;
+  const words_t p = (words_t)reinterpret_cast<uint64_t>(a.items + rfl(i));
+  return WorkItem{p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]};
+}
+
 // The item in each of a kernel's branches by itself: what they share would otherwise be
 // computed ahead of them and held (spilled) for all of them.
 __device__ __forceinline__ WorkItem opaque(WorkItem it) {
@@ -780,14 +787,189 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
   if (h == 0 && cs == 0 && ts == 0) store_lse(a, it, j_, head, M, l_run);
 }
 
+// ================================================================== one wave an item
+// Short items of at most 16 rows (a beam's own tokens), pages of a multiple of 16 tokens:
+// each wave of a workgroup takes an item of its own, in steps of 16 tokens through its
+// share of the stages (as many steps in flight as the others have tiles), with no barrier.
+// Four such items would otherwise be four workgroups that start, wait and end for a tile
+// or two each.  All of a step's tokens lie in one page, so its scales are scalars.
+template <typename T, int D>
+__device__ __forceinline__ void wave_item(const AttnArgs& a, const WorkItem& item, TileShared<D>& sh, int w) {
+  const WorkItem it = opaque(item);
+  constexpr int CPR = D / 16, RPI = 64 / CPR, IPW = 16 / RPI, NST = TileShared<D>::kStages;
+  constexpr int PLANE = 16 * D, STEP = 2 * PLANE, OPS = 2 * IPW;
+  constexpr int KP = D / 64, MT = D / 16;
+  const int kvh = blockIdx.y, lane = threadIdx.x & 63, lg = lane >> 4, lc = lane & 15;
+  const int g = a.g, R = it.q_count * g, ps = a.page_size;
+  unsigned char* ring = sh.stage + w * NST * STEP;
+  const uint32_t lds0 = lds_addr(ring);
+
+  // ---- page ids (with Q), then scales and the first steps
+  const int slot0 = it.tok_begin - it.first_page * ps;
+  const int n_pages = (int)(((float)(slot0 + it.tok_count - 1) + 0.5f) * (1.f / (float)ps)) + 1;
+  const int id = a.pages[it.page_begin + it.first_page + min(lane, n_pages - 1)];
+  const int row = lc, j = (int)(((float)row + 0.5f) * (1.f / (float)g)), hh = row - j * g;
+  v8s qf[2 * KP];
+  if (row < R) {
+    const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(it.q_begin + j) * a.q_sn + (int64_t)(kvh * g + hh) * a.q_sh;
+#pragma unroll
+    for (int x = 0; x < 2 * KP; ++x) qf[x] = *reinterpret_cast<const v8s*>(qp + 16 * (4 * (x >> 1) + lg) + 8 * (x & 1));
+  } else {
+#pragma unroll
+    for (int x = 0; x < 2 * KP; ++x) qf[x] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int x = 0; x < 2 * KP; ++x) asm volatile("" : "+v"(qf[x]));
+  const uint8_t* sp = a.kv_scale + (int64_t)id * 2 * a.hkv + kvh;
+  const int k_byte = sp[0], v_byte = sp[a.hkv];
+  const uint32_t row_bytes = (uint32_t)a.hkv * D, vplane = (uint32_t)ps * row_bytes, page_bytes = 2 * vplane;
+  const uint64_t kvb = reinterpret_cast<uint64_t>(a.kv) + (uint64_t)kvh * D;
+  uint32_t off[IPW];
+#pragma unroll
+  for (int i = 0; i < IPW; ++i) {
+    const int r = i * RPI + lane / CPR;
+    off[i] = (uint32_t)r * row_bytes + ((uint32_t)((lane % CPR) ^ swz<CPR>(r)) << 4);
+  }
+  const int steps = (it.tok_count + 15) >> 4;
+  int l_page = 0, l_slot = slot0, l_tok = 0;           // of the next step to load
+  auto load = [&](uint32_t dst) {
+    const uint32_t pid = (uint32_t)__builtin_amdgcn_readlane(id, l_page);
+    const uint64_t base = kvb + (uint64_t)pid * page_bytes + (uint32_t)l_slot * row_bytes;
+    const int left = it.tok_count - 1 - l_tok;         // rows of this step up to the item's last token
+    if (left >= 15) {
+#pragma unroll
+      for (int i = 0; i < IPW; ++i) dma16_s(base, off[i], dst + i * 1024);
+#pragma unroll
+      for (int i = 0; i < IPW; ++i) dma16_s(base + vplane, off[i], dst + PLANE + i * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < IPW; ++i) {
+        const int r = i * RPI + lane / CPR;
+        const uint64_t src = base + (uint32_t)min(r, left) * row_bytes + ((uint32_t)((lane % CPR) ^ swz<CPR>(r)) << 4);
+        stream::dma16(reinterpret_cast<const void*>(src), dst + i * 1024);
+        stream::dma16(r <= left ? reinterpret_cast<const void*>(src + vplane) : &kZeroChunk, dst + PLANE + i * 1024);
+      }
+    }
+    l_tok += 16;
+    l_slot += 16;
+    if (l_slot >= ps) {
+      l_slot -= ps;
+      ++l_page;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NST; ++i)
+    if (i < steps) load(lds0 + i * STEP);
+
+  // ---- operand offsets
+  uint32_t koff[KP];
+#pragma unroll
+  for (int kp = 0; kp < KP; ++kp) koff[kp] = lc * D + (((4 * kp + lg) ^ swz<CPR>(lc)) << 4);
+  const int vr = 4 * lg + ((lc >> 1) & 3);             // (a transposed read takes 8 rows: these four, twice)
+  float m_run = -INFINITY, l_run = 0.f;
+  v4f o_acc[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) o_acc[mt] = v4f{0.f, 0.f, 0.f, 0.f};
+  int page = 0, slot = slot0, st = 0;
+  for (int step = 0; step < steps; ++step, st = st + 1 == NST ? 0 : st + 1) {
+    // this step's loads have landed, those of up to NST - 1 newer ones may be in flight
+    const int newer = min(NST - 1, steps - 1 - step);
+    if (newer == 0) __builtin_amdgcn_s_waitcnt(BE_VMCNT(0));
+    else if (newer == 1) __builtin_amdgcn_s_waitcnt(BE_VMCNT(OPS));
+    else __builtin_amdgcn_s_waitcnt(BE_VMCNT(2 * OPS));
+    asm volatile("" ::: "memory");
+    const unsigned char* kt = ring + st * STEP;
+    const unsigned char* vt = kt + PLANE;
+    const float ks = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(k_byte, page) << 23) * a.scale_log2;
+    const float vs = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(v_byte, page) << 23);
+    slot += 16;
+    if (slot >= ps) {
+      slot -= ps;
+      ++page;
+    }
+    v4i kc[KP];
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) kc[kp] = *reinterpret_cast<const v4i*>(kt + koff[kp]);
+    v2i vc[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+      vc[mt] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i_t)(vt + vr * D + ((mt ^ swz<CPR>(vr)) << 4) + (lc & 1) * 8));
+    v4f x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+      x = mfma_qk<T>(codes8<T>(kc[kp][0], kc[kp][1]), qf[2 * kp], x);
+      x = mfma_qk<T>(codes8<T>(kc[kp][2], kc[kp][3]), qf[2 * kp + 1], x);
+    }
+    x *= ks;
+    const int left = it.tok_count - step * 16 - 4 * lg;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r >= left) x[r] = -INFINITY;
+    const float mx = rows4_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+    if (__builtin_amdgcn_ballot_w64(mx > m_run + 8.f) != 0) {         // (as in the 32-row tiles)
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
+      l_run *= alpha;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) o_acc[mt] *= alpha;
+      m_run = m_new;
+    }
+    const float msafe = m_run == -INFINITY ? 0.f : m_run;
+    float p[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      p[r] = __builtin_amdgcn_exp2f(x[r] - msafe);
+      l_run += p[r];
+    }
+    const v4s pf = pack4<T>(p[0], p[1], p[2], p[3]);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+      o_acc[mt] = mfma_pv<T>(__builtin_bit_cast(v4s, (u2){value2<T, false>(vc[mt][0], vs), value2<T, true>(vc[mt][0], vs)}), pf, o_acc[mt]);
+    }
+    if (step + NST < steps) {
+      __builtin_amdgcn_s_waitcnt(0xc07f);              // lgkmcnt(0): this step's reads are done with its stage
+      load(lds0 + st * STEP);
+    }
+  }
+  l_run = rows4_sum(l_run);
+  if (row >= R) return;
+  const int head = kvh * g + hh;
+  const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+  if (it.out_row < 0) {
+    T* op = reinterpret_cast<T*>(a.out) + (int64_t)(it.q_begin + j) * a.o_sn + (int64_t)head * a.o_sh;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+      *reinterpret_cast<v4s*>(op + mt * 16 + 4 * lg) =
+          pack4<T>(o_acc[mt][0] * inv, o_acc[mt][1] * inv, o_acc[mt][2] * inv, o_acc[mt][3] * inv);
+  } else {
+    float* op = a.part_o + ((int64_t)(it.out_row + j) * a.hq + head) * D;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) *reinterpret_cast<v4f*>(op + mt * 16 + 4 * lg) = o_acc[mt] * inv;
+  }
+  if (lg == 0) store_lse(a, it, j, head, m_run, l_run);
+}
+
 // A workgroup takes as many row tiles as its item has: with fewer, the waves share out
 // the tokens of a row tile (and the columns) rather than idle.
 template <typename T, int D, int PG, bool QUADS>
-__global__ __launch_bounds__(256, D == 256 || !QUADS ? 2 : D == 128 ? 3 : 4) void attn_kv8_kernel(AttnArgs a, int first_item) {
+__global__ __launch_bounds__(256, D == 256 || !QUADS ? 2 : D == 128 ? 3 : 4) void attn_kv8_kernel(AttnArgs a, int first_item, int end_item, int waves) {
   __shared__ __attribute__((aligned(1024))) TileShared<D> sh;
-  const int item = (a.live_blocks ? *a.live_blocks : first_item) + (int)blockIdx.x;
-  if (a.live_items && item >= *a.live_items) return;
-  const WorkItem it = a.items[item];
+  // items [first, end - waves) by workgroups, the last `waves` by one wave each
+  if (a.live_blocks) {
+    first_item = a.live_blocks[0];
+    waves = a.live_blocks[kHdrWaves - kHdrBlocks];
+    end_item = *a.live_items;
+  }
+  const int item = first_item + (int)blockIdx.x, singles = end_item - waves;
+  if (item >= singles) {
+    if constexpr (PG == 2) {
+      const int w = rfl(threadIdx.x >> 6), mine = singles + 4 * (item - singles) + w;
+      if (mine < end_item) wave_item<T, D>(a, item_at(a, mine), sh, w);
+    }
+    return;
+  }
+  const WorkItem it = item_at(a, rfl(item));
   const int R = it.q_count * a.g;
   if (R <= 16) {
     tile_item<T, D, 1, PG, QUADS>(a, it, sh);
@@ -803,12 +985,13 @@ __global__ __launch_bounds__(256, D == 256 || !QUADS ? 2 : D == 128 ? 3 : 4) voi
 template <typename T, int D>
 static int launch_tile(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st) {
   const int first = info->num_wg;                    // the block kernel's items come first
-  const dim3 grid(info->static_layout ? info->grid_items : info->grid_items - first, info->num_kv_heads);
+  const int end = info->grid_items, waves = info->num_tail_items;
+  const dim3 grid(info->static_layout ? end : end - first - waves + (waves + 3) / 4, info->num_kv_heads);
   if (grid.x == 0) return BE_OK;
-  if (a.page_size % 16 == 0) attn_kv8_kernel<T, D, 2, true><<<grid, 256, 0, st>>>(a, first);
-  else if (paged4(a.page_size, D)) attn_kv8_kernel<T, D, 1, true><<<grid, 256, 0, st>>>(a, first);
-  else if (a.page_size % 4 == 0) attn_kv8_kernel<T, D, 0, true><<<grid, 256, 0, st>>>(a, first);
-  else attn_kv8_kernel<T, D, 0, false><<<grid, 256, 0, st>>>(a, first);
+  if (a.page_size % 16 == 0) attn_kv8_kernel<T, D, 2, true><<<grid, 256, 0, st>>>(a, first, end, waves);
+  else if (paged4(a.page_size, D)) attn_kv8_kernel<T, D, 1, true><<<grid, 256, 0, st>>>(a, first, end, waves);
+  else if (a.page_size % 4 == 0) attn_kv8_kernel<T, D, 0, true><<<grid, 256, 0, st>>>(a, first, end, waves);
+  else attn_kv8_kernel<T, D, 0, false><<<grid, 256, 0, st>>>(a, first, end, waves);
   BE_HIP_CHECK(hipGetLastError());
   return BE_OK;
 }
@@ -847,7 +1030,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_block_kernel(AttnArgs a, int 
   const int item = (int)blockIdx.x / a.hkv, kvh = (int)blockIdx.x - item * a.hkv;
   if (item >= (a.live_blocks ? *a.live_blocks : n_items)) return;
 
-  const WorkItem it = a.items[item];
+  const WorkItem it = item_at(a, item);
   const int tid = threadIdx.x;
   const int w = rfl(tid >> 6), lane = tid & 63, h = lane >> 5, lr = lane & 31;
   const int g = a.g, R = it.q_count * g, ps = a.page_size;

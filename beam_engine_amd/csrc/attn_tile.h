@@ -264,6 +264,9 @@ int f32_launch(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st)
 int kv8_launch(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st);
 constexpr int kMaxPageKv8 = 1024;      // tokens of a page of an 8-bit cache
 constexpr int kMaxPagesKv8 = 256;      // pages of an item
+// Items of at most 16 rows and this many tokens, in pages of a multiple of 16 tokens and
+// without a causal mask, take a wave each.
+constexpr int kWaveTokens = 128;
 // Rows of its items: above 64 the block kernel's.
 inline int kv8_max_rows(int head_dim) { return head_dim == 256 ? 64 : kMaxTileRows; }
 

@@ -312,7 +312,7 @@ typedef struct be_attn_plan_info {
   /* With BE_PLAN_TAIL_ROLE, the tail chunks are attended by tail-role
    * workgroups of the streaming kernel instead: items [n][8] (query, KV head,
    * first tail entry, entries, slot) whose results join the records as slots. */
-  int32_t num_tail_items;
+  int32_t num_tail_items;  /* (kernel 4: items that one wave each takes, which come last) */
   int32_t off_tail_items;
   int32_t stream_loop;     /* streaming kernel's loop: 0 direct global->LDS loads, 1 register-staged;
                               2: causal groups as 128-row blocks (the tile kernels' plan layout) */
