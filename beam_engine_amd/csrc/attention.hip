@@ -247,26 +247,37 @@ __global__ __launch_bounds__(256) void merge2_kernel(const float* oa, const floa
 // Query tiles and key chunks of an 8-bit cache's plan: the longest items' chain, the CUs'
 // shares of the tiles, partial rows and the merge are weighed against each other for
 // both row limits (tile kernel only, or 128-row blocks for what exceeds 64 rows) and
-// chunks of 1 to 1024 tiles, and the shortest estimate wins.
+// the longest items in 1 to 1024 chunks, and the shortest estimate wins.
 struct Kv8Cut {
   int rows_cap;
   int64_t chunk;           // tokens
   double us;
 };
-// Microseconds at head_dim 128 (kv8_scale for others), MI355X: a 64-token tile of a CU's
-// share, the same for a workgroup that has the CU to itself, a workgroup's start and end
-// as latency and as the CU's time; [0] up to 64 rows, [1] blocks.
-constexpr double kKv8Tile[2] = {1.0, 1.35}, kKv8Alone[2] = {0.9, 1.6}, kKv8Start[2] = {5.0, 6.0}, kKv8Wg[2] = {0.8, 1.5};
+// Microseconds on MI355X at head_dim 128 (kv8_scale for others), fitted to 280 timed cuts
+// of 16 shapes: a 64-token tile of a CU's share and the same for a workgroup that has
+// the CU to itself, a workgroup's start and end as the CU's time; [0] up to 64 rows,
+// [1] blocks.  The cuts they choose are 2 % behind the fastest on average, 11 % at worst;
+// a fixed chunk of 512 tokens is 11 % behind on average and 67 % at worst.  Blocks take
+// 97 us against 104 (8 prompts of 1024 tokens, 32 heads of 128 over 8) and 61 against 70
+// (4 x 128 tokens onto 4096), but 219 against 178 where 512 rows share a prefix of 32768
+// tokens (64 heads over 8) and 51 against 39 at 4096: there the tiles' workgroups, three
+// a CU rather than two, find each other's keys in L2.
+constexpr double kKv8Tile[2] = {0.47, 1.1}, kKv8Alone[2] = {0.63, 1.6}, kKv8Wg[2] = {1.5, 0.45};
+constexpr double kKv8Wave = 0.11;      // four items of a wave each
+constexpr double kKv8Start = 0.62, kKv8Launch = 12.0, kKv8Both = 6.5, kKv8Merge = 1.0;
+constexpr double kKv8Part = 2.6e6;     // bytes of partial outputs a microsecond
+constexpr double kKv8Tail = 0.17;      // of the longest item's time, where items wait for CUs
 constexpr int kKv8Slots[2] = {3, 2};
-static double kv8_scale(int d) { return 0.35 + 0.65 * d / 128; }
+static double kv8_scale(int d) { return 0.6 + 0.4 * d / 128; }
 
-template <typename Vis>
-static Kv8Cut kv8_cut(const std::vector<Group>& groups, const Vis& vis, int g, int hq, int hkv, int d, int num_cus, int only_rows) {
+template <typename Vis, typename Causal>
+static Kv8Cut kv8_cut(const std::vector<Group>& groups, const Vis& vis, const Causal& is_causal, int g, int hkv, int d, int page_size, int num_cus, int only_rows) {
   const double per_d = kv8_scale(d);
   Kv8Cut best{0, 0, 0};
   struct Tile {            // query tiles of a plan: 64-token tiles of keys, rows, how many such
     int64_t tiles;
     int rows;
+    bool wave;             // takes a wave each, if uncut
     int64_t n;
   };
   for (int rows_cap : {64, kMaxTileRows}) {
@@ -278,23 +289,32 @@ static Kv8Cut kv8_cut(const std::vector<Group>& groups, const Vis& vis, int g, i
       if (gr.kv_len <= 0) continue;
       for (int qa = gr.q0; qa < gr.q1; qa += q_tile) {
         const int qn = std::min(q_tile, gr.q1 - qa);
-        const int64_t t = ceil_div(vis(gr, qa + qn - 1), kTile);
+        const int64_t seen = vis(gr, qa + qn - 1), t = ceil_div(seen, kTile);
         if (t == 0) continue;
         longest = std::max(longest, t);
         // (the last tile of a group of blocks is a block too)
         const int rows = std::min(q_tile, gr.q1 - gr.q0) * g;
-        if (!qt.empty() && qt.back().tiles == t && qt.back().rows == rows) ++qt.back().n;
-        else qt.push_back(Tile{t, rows, 1});
+        const bool wave = !is_causal(gr) && qn * g <= 16 && rows <= 64 && seen <= kWaveTokens && page_size % 16 == 0;
+        if (!qt.empty() && qt.back().tiles == t && qt.back().rows == rows && qt.back().wave == wave) ++qt.back().n;
+        else qt.push_back(Tile{t, rows, wave, 1});
       }
     }
     if (qt.empty()) return Kv8Cut{rows_cap, kTile, 0};
-    for (int64_t c = 1; c <= 1024; c = c < 4 ? c + 1 : c * 5 / 4) {
-      double work[2] = {0, 0}, wgs[2] = {0, 0}, part = 0;
+    int64_t last = 0;
+    for (int64_t n = 1; n <= 1024; n = n < 8 ? n + 1 : n * 9 / 8) {
+      const int64_t c = ceil_div(longest, n);
+      if (c == last) continue;
+      last = c;
+      double work[2] = {0, 0}, wgs[2] = {0, 0}, waves = 0, part = 0;
       int64_t chain[2] = {0, 0};
       bool split = false;
       for (const Tile& x : qt) {
         const int k = x.rows > 64;
         const int64_t nch = ceil_div(x.tiles, c);
+        if (x.wave && nch == 1) {
+          waves += (double)x.n * hkv / 4;
+          continue;
+        }
         work[k] += (double)x.tiles * x.n * hkv;
         wgs[k] += (double)nch * x.n * hkv;
         chain[k] = std::max(chain[k], std::min(c, x.tiles));
@@ -303,19 +323,18 @@ static Kv8Cut kv8_cut(const std::vector<Group>& groups, const Vis& vis, int g, i
           part += (double)nch * x.n * x.rows * hkv * d * 4;
         }
       }
-      double us = 3.0;
+      double us = kKv8Launch;
       for (int k = 0; k < 2; ++k) {
         if (wgs[k] == 0) continue;
         const double per_cu = wgs[k] / num_cus, slots = kKv8Slots[k], tile = kKv8Tile[k] * per_d;
-        const double share = (work[k] * tile + wgs[k] * kKv8Wg[k]) / num_cus + part / 5e6;
-        const double busy = std::min(slots, std::ceil(per_cu));
-        const double line = kKv8Start[k] + chain[k] * std::max(kKv8Alone[k] * per_d, busy * tile);
-        // the last generation of workgroups runs with what it leaves idle
-        us += std::max(share, line) + (per_cu > slots ? 0.5 * kKv8Start[k] : 0.0) + (k == 1 && wgs[0] > 0 ? 2.5 : 0.0);
+        const double share = (work[k] * tile + wgs[k] * kKv8Wg[k] + (k == 0 ? waves * kKv8Wave : 0.0)) / num_cus;
+        const double line = kKv8Start + chain[k] * std::max(kKv8Alone[k] * per_d, std::min(slots, std::ceil(per_cu)) * tile);
+        us += std::max(share + (per_cu > slots ? kKv8Tail * line : 0.0), line);
       }
-      if (split) us += 3.0 + part / 5e6;
+      if (wgs[1] > 0 && wgs[0] + waves > 0) us += kKv8Both;
+      if (split) us += kKv8Merge + part / kKv8Part;
       if (best.rows_cap == 0 || us < best.us) best = Kv8Cut{rows_cap, c * kTile, us};
-      if (c >= longest) break;
+      if (c == 1) break;
     }
   }
   return best;
@@ -475,7 +494,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   }
   int64_t kv8_chunk = 0;
   if (kv8) {
-    const Kv8Cut cut = kv8_cut(groups, vis, g, hq, hkv, d, num_cus, caps || rows_cap < 64 || g > 64 ? rows_cap : 0);
+    const Kv8Cut cut = kv8_cut(groups, vis, is_causal, g, hkv, d, page_size, num_cus, caps || rows_cap < 64 || g > 64 ? rows_cap : 0);
     if (cut.rows_cap) {
       rows_cap = cut.rows_cap;
       kv8_chunk = cut.chunk;
@@ -841,6 +860,7 @@ int attn_run(const be_attn_plan_info* info, const int32_t* plan, void* partials,
   a.pages = plan + info->off_pages;
   a.page_size = info->page_size;
   a.hkv = info->num_kv_heads;
+  a.hkv_inv = (uint32_t)((0xffffffffull + a.hkv) / a.hkv);
   a.hq = info->num_qo_heads;
   a.g = info->num_qo_heads / info->num_kv_heads;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
@@ -853,7 +873,11 @@ int attn_run(const be_attn_plan_info* info, const int32_t* plan, void* partials,
                    ? reinterpret_cast<int32_t*>(reinterpret_cast<char*>(partials) + info->counter_offset)
                    : nullptr;
   int rc = BE_OK;
-  if (info->kernel == 4) BE_REQUIRE(rows_aligned(info, a), "rows of q, out and an 8-bit cache must start on 16 bytes");
+  if (info->kernel == 4) {
+    BE_REQUIRE(rows_aligned(info, a), "rows of q, out and an 8-bit cache must start on 16 bytes");
+    BE_REQUIRE((int64_t)info->grid_items * info->num_kv_heads < (1 << 24), "%d work items of %d KV heads exceed a launch",
+               info->grid_items, info->num_kv_heads);
+  }
   if ((phases & BE_RUN_ATTENTION) && info->grid_items > 0) {
     if (info->kernel == 4) rc = kv8_launch(info, a, st);
     else switch (info->dtype) {

@@ -263,6 +263,15 @@ struct Codes {
   }
 };
 
+// Consecutive workgroups are the KV heads of one item: an XCD keeps the same heads in its
+// L2, and the items start in their order.  x / hkv by the reciprocal, which is at most
+// one too large (a division by a variable costs a start some 200 cycles).
+__device__ __forceinline__ int item_of(const AttnArgs& a, uint32_t x) {
+  if (a.hkv == 1) return (int)x;
+  const uint32_t i = __umulhi(x, a.hkv_inv);
+  return (int)(i * (uint32_t)a.hkv > x ? i - 1 : i);
+}
+
 // An item's record by scalar loads, whatever the compiler can tell of its index.
 __device__ __forceinline__ WorkItem item_at(const AttnArgs& a, int i) {
   typedef const int32_t __attribute__((address_space(4)))* words_t;
@@ -278,7 +287,7 @@ __device__ __forceinline__ WorkItem opaque(WorkItem it) {
 }
 
 template <typename T, int D, int RT, int PG, bool QUADS>
-__device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& item, TileShared<D>& sh) {
+__device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& item, int kvh, TileShared<D>& sh) {
   const WorkItem it = opaque(item);
   constexpr int CPR = D / 16;                        // 16-code chunks of a row
   using Loader = Codes<D, PG, swz<CPR>>;
@@ -293,7 +302,6 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& ite
 
   unsigned char* stage = sh.stage;
   int32_t* nan_tok = sh.nan_tok;
-  const int kvh = blockIdx.y;
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));
   const int w = rfl(tid >> 6), lane = tid & 63, lg = lane >> 4, lc = lane & 15;
@@ -546,7 +554,7 @@ __device__ __forceinline__ int swz32(int r) {
 // eight registers at a time, the B operand of Oᵀ += Vᵀ Pᵀ over the token order that the
 // transposed V reads follow.
 template <typename T, int D, int RT, int PG, bool QUADS>
-__device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& item, TileShared<D>& sh) {
+__device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& item, int kvh, TileShared<D>& sh) {
   const WorkItem it = opaque(item);
   constexpr int CPR = D / 16;                        // 16-code chunks of a row
   using Loader = Codes<D, PG, swz32<CPR>>;
@@ -561,7 +569,6 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
   static_assert(4 * COMB_SLOT <= NST * STAGE, "combine scratch must fit");
 
   unsigned char* stage = sh.stage;
-  const int kvh = blockIdx.y;
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));
   const int w = rfl(tid >> 6), lane = tid & 63, h = lane >> 5, lr = lane & 31;
@@ -794,12 +801,12 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
 // Four such items would otherwise be four workgroups that start, wait and end for a tile
 // or two each.  All of a step's tokens lie in one page, so its scales are scalars.
 template <typename T, int D>
-__device__ __forceinline__ void wave_item(const AttnArgs& a, const WorkItem& item, TileShared<D>& sh, int w) {
+__device__ __forceinline__ void wave_item(const AttnArgs& a, const WorkItem& item, int kvh, TileShared<D>& sh, int w) {
   const WorkItem it = opaque(item);
   constexpr int CPR = D / 16, RPI = 64 / CPR, IPW = 16 / RPI, NST = TileShared<D>::kStages;
   constexpr int PLANE = 16 * D, STEP = 2 * PLANE, OPS = 2 * IPW;
   constexpr int KP = D / 64, MT = D / 16;
-  const int kvh = blockIdx.y, lane = threadIdx.x & 63, lg = lane >> 4, lc = lane & 15;
+  const int lane = threadIdx.x & 63, lg = lane >> 4, lc = lane & 15;
   const int g = a.g, R = it.q_count * g, ps = a.page_size;
   unsigned char* ring = sh.stage + w * NST * STEP;
   const uint32_t lds0 = lds_addr(ring);
@@ -961,24 +968,24 @@ __global__ __launch_bounds__(256, D == 256 || !QUADS ? 2 : D == 128 ? 3 : 4) voi
     waves = a.live_blocks[kHdrWaves - kHdrBlocks];
     end_item = *a.live_items;
   }
-  const int item = first_item + (int)blockIdx.x, singles = end_item - waves;
+  const int wg = item_of(a, blockIdx.x), kvh = (int)blockIdx.x - wg * a.hkv, item = first_item + wg, singles = end_item - waves;
   if (item >= singles) {
     if constexpr (PG == 2) {
       const int w = rfl(threadIdx.x >> 6), mine = singles + 4 * (item - singles) + w;
-      if (mine < end_item) wave_item<T, D>(a, item_at(a, mine), sh, w);
+      if (mine < end_item) wave_item<T, D>(a, item_at(a, mine), kvh, sh, w);
     }
     return;
   }
   const WorkItem it = item_at(a, rfl(item));
   const int R = it.q_count * a.g;
   if (R <= 16) {
-    tile_item<T, D, 1, PG, QUADS>(a, it, sh);
+    tile_item<T, D, 1, PG, QUADS>(a, it, kvh, sh);
   } else if constexpr (D == 256) {                   // (32-row tiles would not fit the registers)
-    if (R <= 32) tile_item<T, D, 2, PG, QUADS>(a, it, sh);
-    else tile_item<T, D, 4, PG, QUADS>(a, it, sh);
+    if (R <= 32) tile_item<T, D, 2, PG, QUADS>(a, it, kvh, sh);
+    else tile_item<T, D, 4, PG, QUADS>(a, it, kvh, sh);
   } else {
-    if (R <= 32) tile32_item<T, D, 1, PG, QUADS>(a, it, sh);
-    else tile32_item<T, D, 2, PG, QUADS>(a, it, sh);
+    if (R <= 32) tile32_item<T, D, 1, PG, QUADS>(a, it, kvh, sh);
+    else tile32_item<T, D, 2, PG, QUADS>(a, it, kvh, sh);
   }
 }
 
@@ -986,8 +993,8 @@ template <typename T, int D>
 static int launch_tile(const be_attn_plan_info* info, const AttnArgs& a, hipStream_t st) {
   const int first = info->num_wg;                    // the block kernel's items come first
   const int end = info->grid_items, waves = info->num_tail_items;
-  const dim3 grid(info->static_layout ? end : end - first - waves + (waves + 3) / 4, info->num_kv_heads);
-  if (grid.x == 0) return BE_OK;
+  const unsigned grid = (unsigned)(info->static_layout ? end : end - first - waves + (waves + 3) / 4) * info->num_kv_heads;
+  if (grid == 0) return BE_OK;
   if (a.page_size % 16 == 0) attn_kv8_kernel<T, D, 2, true><<<grid, 256, 0, st>>>(a, first, end, waves);
   else if (paged4(a.page_size, D)) attn_kv8_kernel<T, D, 1, true><<<grid, 256, 0, st>>>(a, first, end, waves);
   else if (a.page_size % 4 == 0) attn_kv8_kernel<T, D, 0, true><<<grid, 256, 0, st>>>(a, first, end, waves);
@@ -1026,8 +1033,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_block_kernel(AttnArgs a, int 
   __shared__ uint16_t sc_lds[kMaxPagesKv8];          // scale bytes of the pages: K | V << 8
   __shared__ int32_t nan_tok[D];
   __shared__ int32_t nan_any, k_top;
-  // consecutive workgroups are the KV heads of one item: an XCD keeps the same heads in its L2
-  const int item = (int)blockIdx.x / a.hkv, kvh = (int)blockIdx.x - item * a.hkv;
+  const int item = item_of(a, blockIdx.x), kvh = (int)blockIdx.x - item * a.hkv;
   if (item >= (a.live_blocks ? *a.live_blocks : n_items)) return;
 
   const WorkItem it = item_at(a, item);

@@ -56,6 +56,7 @@ struct AttnArgs {
   const int32_t* live_items;   // fixed layout: live item count (surplus workgroups exit)
   const int32_t* live_blocks;  // fixed layout of an 8-bit cache: how many of them are blocks
   int page_size, hkv, hq, g;
+  uint32_t hkv_inv;   // 8-bit caches: ceil(2^32 / hkv)
   float scale_log2;   // sm_scale * log2(e)
 };
 
