@@ -104,6 +104,7 @@ class PlanStats:
         self.kernel = {0: "valu", 1: "tile", 2: "stream", 3: "rows", 4: "kv8"}[int(info.kernel)]
         self.num_tails = int(info.num_tails) if self.kernel == "stream" else 0
         self.chunk_tokens = int(info.chunk_tokens)
+        self.launches = ()
         merge = (int(info.grid_merge) > 0 and not info.fused_merge) or int(info.grid_zero) > 0
         if self.kernel == "rows":
             self.launches = ("attn_rows_kernel",)
@@ -111,13 +112,16 @@ class PlanStats:
             self.launches = ("attn_stream_kernel",) + (("tail_merge_kernel",) if info.grid_merge > 0 else ())
         else:
             rows = int(info.tile_rows)
-            if info.kernel == 4:
-                name = "attn_kv8_kernel"
+            if info.kernel == 4:      # the block kernel's items (a fixed layout may hold both kinds), then the others
+                blocks, rest = int(info.num_wg) > 0, info.static_layout or info.grid_items > info.num_wg
+                name = "attn_kv8_block_kernel" if blocks else "attn_kv8_kernel"
+                if blocks and rest:
+                    self.launches = ("attn_kv8_kernel",)
             elif info.kernel == 0:
                 name = "attn_f32_kernel" if rows and info.dtype == _lib.dtype_code(torch.float32) else "attn_valu_kernel"
             else:
                 name = "attn_block_kernel" if rows == 128 and int(info.head_dim) <= 128 else "attn_tile_kernel"
-            self.launches = (name,) + (("merge_kernel",) if merge else ())
+            self.launches = (name,) + self.launches + (("merge_kernel",) if merge else ())
 
     @property
     def bytes(self) -> int:

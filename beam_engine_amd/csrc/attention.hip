@@ -361,7 +361,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
     if (g > kv8_max_rows(d)) return fail(BE_ERR_UNSUPPORTED, "GQA group %d exceeds %d (8-bit cache)", g, kv8_max_rows(d));
     if (page_size > kMaxPageKv8) return fail(BE_ERR_UNSUPPORTED, "page size %d exceeds %d (8-bit cache)", page_size, kMaxPageKv8);
     if (flags & (BE_PLAN_FORCE_VALU | BE_PLAN_FUSED_MERGE | BE_PLAN_ROWS))
-      return fail(BE_ERR_UNSUPPORTED, "plan flags %d: an 8-bit cache has one kernel, with a separate merge", flags);
+      return fail(BE_ERR_UNSUPPORTED, "plan flags %d: an 8-bit cache has kernels of its own, with a separate merge", flags);
   }
 
   // ---- validate levels, collect groups
@@ -494,7 +494,7 @@ int attn_plan(const be_level* levels, int num_levels, int num_queries, int hq, i
   }
   int64_t kv8_chunk = 0;
   if (kv8) {
-    const Kv8Cut cut = kv8_cut(groups, vis, is_causal, g, hkv, d, page_size, num_cus, caps || rows_cap < 64 || g > 64 ? rows_cap : 0);
+    const Kv8Cut cut = kv8_cut(groups, vis, is_causal, g, hkv, d, page_size, num_cus, caps || g > 64 ? rows_cap : flags & BE_PLAN_NO_BLOCKS ? 64 : 0);
     if (cut.rows_cap) {
       rows_cap = cut.rows_cap;
       kv8_chunk = cut.chunk;

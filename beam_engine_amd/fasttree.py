@@ -156,26 +156,30 @@ def prepare_fasttree_metadata_for_paged_cache(tree_info: Sequence, req_to_token,
                                               device: str = "cuda", *, page_size: int = 16,
                                               q_data_type=torch.bfloat16,
                                               workspace: Optional[torch.Tensor] = None,
-                                              costs: str = "fasttree") -> FastTreeMetadata:
+                                              costs: str = "fasttree", kv_data_type=None) -> FastTreeMetadata:
     """Drop-in for preparation.py:11-225 (same leading arguments): plans the
     step's tree attention once for every layer.  ``page_size`` is the page
     table's (the reference's kernel reads slots, the plan reads pages);
     ``workspace`` a device byte buffer for the plan and its partials (a
-    shared 128 MB one per device by default)."""
+    shared 128 MB one per device by default); ``kv_data_type`` the cache's, where
+    that is 8 bits (``torch.float8_e4m3fn``)."""
     levels = fasttree_levels(tree_info, req_to_token, batch_size, num_qo_heads, num_kv_heads, page_size, costs)
     ws = workspace if workspace is not None else _workspace(device)
     w = MultiLevelCascadeAttentionWrapper(max(1, len(levels)), ws)
     w.plan([l[0] for l in levels], [l[1] for l in levels], [l[2] for l in levels], [l[3] for l in levels],
-           num_qo_heads, num_kv_heads, head_dim, page_size, causal=False, q_data_type=q_data_type)
+           num_qo_heads, num_kv_heads, head_dim, page_size, causal=False, q_data_type=q_data_type,
+           kv_data_type=kv_data_type)
     return FastTreeMetadata(w, levels, num_qo_heads, num_kv_heads, head_dim)
 
 
 def fasttree_decode(q: torch.Tensor, paged_kv_cache: torch.Tensor, o: Optional[torch.Tensor],
-                    metadata: FastTreeMetadata, sm_scale: Optional[float] = None) -> torch.Tensor:
+                    metadata: FastTreeMetadata, sm_scale: Optional[float] = None, *,
+                    kv_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Drop-in for kernel.py:288-348: o[i] = attention of q[i] ([N, Hq, D])
     over candidate i's whole path in the layer's paged cache ``[P, 2,
     page_size, Hkv, D]`` (the reference passes K / V buffer copies instead).
-    ``sm_scale`` must be D^-1/2 (the plan's scale) when given."""
+    ``sm_scale`` must be D^-1/2 (the plan's scale) when given; ``kv_scale``
+    the layer's scales, with a cache of 8 bits."""
     if sm_scale is not None and abs(sm_scale - metadata.head_dim ** -0.5) > 1e-12 * sm_scale:
         raise NotImplementedError("fasttree_decode runs at sm_scale = head_dim ** -0.5")
-    return metadata.wrapper.run(q, paged_kv_cache, out=o)
+    return metadata.wrapper.run(q, paged_kv_cache, out=o, kv_scale=kv_scale)

@@ -84,6 +84,9 @@ class BatchedBeamSearch:
         self.device = page_table.device
         # an 8-bit cache: the attention plans name its type, and each layer's run its scales
         self._kv_type = page_table.store_dtype if page_table.kv8 else None
+        if page_table.kv8 and getattr(model, "dtype", page_table.compute_dtype) != page_table.compute_dtype:
+            raise ValueError(f"the model computes in {model.dtype}, the page table's compute_dtype is "
+                             f"{page_table.compute_dtype}")
         # the trie and its pages live in native code: one call per selection,
         # one for the step's metadata and attention plan (any strategy kind)
         self.state = NativeBeamState(beam_size, page_table)

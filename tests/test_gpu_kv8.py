@@ -554,6 +554,249 @@ def test_offsets_beyond_32_bits():
     close(o, want, tol, "far pages")
 
 
+# ------------------------------------------------------------------ each kernel
+def blocks_of(w):
+    return int(w._info.num_wg)
+
+
+def planned(kind, qo, ptr, ind, last, hq, hkv, d, page, dtype, causal, **kw):
+    """A prefill wrapper whose items of more than 64 rows are ``kind``: "blocks" (through a
+    fixed layout, which says so), or "tiles" (none has more)."""
+    from beam_engine_amd import BatchPrefillWithPagedKVCacheWrapper
+    w = BatchPrefillWithPagedKVCacheWrapper(workspace(256))
+    if kind == "blocks":
+        w.use_fixed_layout(4096, max(1, qo[-1]), 4096, max(1, qo[-1]), 8192, max(1, qo[-1]), 128)
+    else:
+        w._no_blocks = True
+    w.plan(qo, ptr, ind, last, hq, hkv, d, page, causal=causal, q_data_type=dtype, kv_data_type=F8, **kw)
+    assert w.stats.kernel == "kv8" and (blocks_of(w) > 0) == (kind == "blocks")
+    assert w.stats.launches[0] == ("attn_kv8_block_kernel" if kind == "blocks" else "attn_kv8_kernel")
+    return w
+
+
+@pytest.mark.parametrize("kind", ["tiles", "blocks"])
+@pytest.mark.parametrize("sm_scale", [None, 0.0, -0.11])
+@pytest.mark.parametrize("hq,hkv,d,dtype,page", [
+    (32, 8, 128, torch.bfloat16, 16), (32, 8, 128, torch.float16, 8), (8, 8, 64, torch.float16, 48), (12, 2, 64, torch.bfloat16, 5),
+    (40, 2, 128, torch.float16, 3)])
+def test_tiles_and_blocks(kind, sm_scale, hq, hkv, d, dtype, page):
+    """Prompts of every size through one kernel and the other: a group without queries, one
+    without keys, rows that see nothing, NaN codes in void slots and in V."""
+    say(f"{kind} {hq}/{hkv} d {d} {dtype} page {page} scale {sm_scale}")
+    lens = [(200, 0), (0, 30), (33, 700), (40, -13), (3, 0), (65, 64), (5, -5), (17, 1100)]
+    total, ptr, ind, last, slots = lists([a + c for a, c in lens], page, random.Random(page))
+    codes, scale = cache(total, page, hkv, d, page, spread=3)
+    raw = codes.view(torch.uint8)
+    raw[(raw & 127) == 127] = 3
+    live = torch.zeros(total * page, dtype=torch.bool)
+    live[[t for s in slots for t in s]] = True
+    void = ~live.reshape(total, page).cuda()
+    raw.copy_(torch.where(void[:, None, :, None, None], torch.full_like(raw, 255), raw))
+    t = slots[0][150]
+    raw[t // page, 1, t % page, hkv - 1, d - 3] = 127          # seen by the first prompt's rows from 150 on
+    qo = [0]
+    for a, _ in lens:
+        qo.append(qo[-1] + a)
+    q = torch.randn((qo[-1], hq, d), generator=torch.Generator(device="cuda").manual_seed(d), device="cuda").to(dtype)
+    for causal in (True, False):
+        w = planned(kind, qo, ptr, ind, last, hq, hkv, d, page, dtype, causal, sm_scale=sm_scale)
+        o, lse = w.run(q, codes, kv_scale=scale, return_lse=True)
+        for i, (a, c) in enumerate(lens):
+            if a == 0:
+                continue
+            sees = torch.arange(a, device="cuda") + c + 1 if causal else None
+            want, wl, tol = attend(q[qo[i]:qo[i + 1]], codes, scale, slots[i], sees, sm_scale)
+            close(o[qo[i]:qo[i + 1]], want, tol, f"prompt {i} causal {causal}")
+            lse_close(lse[qo[i]:qo[i + 1]], wl, d, f"prompt {i}")
+
+
+@pytest.mark.parametrize("hq,hkv,page", [(96, 1, 16), (128, 1, 8), (260, 4, 5)])
+def test_groups_beyond_a_tile(hq, hkv, page):
+    """GQA groups of more than 64 heads: blocks alone, whatever the plan."""
+    from beam_engine_amd import BatchDecodeWithPagedKVCacheWrapper
+    say(f"group {hq // hkv}")
+    d, lens, dtype = 128, [1, 0, 17, 500, 2300], torch.bfloat16
+    total, ptr, ind, last, slots = lists(lens, page, random.Random(1))
+    codes, scale = cache(total, page, hkv, d, 3, spread=3)
+    q = torch.randn((len(lens), hq, d), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    for no_blocks in (False, True):
+        w = BatchDecodeWithPagedKVCacheWrapper(workspace())
+        w._no_blocks = no_blocks
+        w.plan(ptr, ind, last, hq, hkv, d, page, q_data_type=dtype, kv_data_type=F8)
+        assert blocks_of(w) == w.stats.num_items
+        o, lse = w.run(q, codes, kv_scale=scale, return_lse=True)
+        for i in range(len(lens)):
+            want, wl, tol = attend(q[i:i + 1], codes, scale, slots[i])
+            close(o[i:i + 1], want, tol, f"len {lens[i]}")
+            lse_close(lse[i:i + 1], wl, d, f"len {lens[i]}")
+
+
+@pytest.mark.parametrize("page", [8, 16, 32])
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(32, 8, 128, torch.bfloat16), (8, 8, 64, torch.float16), (32, 2, 256, torch.bfloat16)])
+def test_waves_of_short_items(hq, hkv, d, dtype, page):
+    """Many short groups of at most 16 rows, a wave each where pages allow: every length
+    around a step, several queries a group, NaN behind each group's last token."""
+    from beam_engine_amd import BatchPrefillWithPagedKVCacheWrapper
+    say(f"waves {hq}/{hkv} d {d} {dtype} page {page}")
+    lens = [n for n in (1, 2, 15, 16, 17, 31, 32, 33, 47, 48, 49, 64, 65, 100, 127, 128, 129)] * 3
+    total, ptr, ind, last, slots = lists(lens, page, random.Random(page))
+    codes, scale = cache(total, page, hkv, d, page, spread=3)
+    raw = codes.view(torch.uint8)
+    live = torch.zeros(total * page, dtype=torch.bool)
+    live[[t for s in slots for t in s]] = True
+    void = ~live.reshape(total, page).cuda()
+    raw[(raw & 127) == 127] = 3
+    raw.copy_(torch.where(void[:, None, :, None, None], torch.full_like(raw, 127), raw))
+    per = max(1, 16 // (hq // hkv))
+    qo = [0]
+    for i in range(len(lens)):
+        qo.append(qo[-1] + (i % per if i % 5 == 0 else 1 + i % per))
+    q = torch.randn((qo[-1], hq, d), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    w = BatchPrefillWithPagedKVCacheWrapper(workspace())
+    w.plan(qo, ptr, ind, last, hq, hkv, d, page, causal=False, q_data_type=dtype, kv_data_type=F8)
+    if page % 16 == 0:
+        assert w._info.num_tail_items >= len(lens) // 2
+    else:
+        assert w._info.num_tail_items == 0
+    o, lse = w.run(q, codes, kv_scale=scale, return_lse=True)
+    for i in range(len(lens)):
+        if qo[i] == qo[i + 1]:
+            continue
+        want, wl, tol = attend(q[qo[i]:qo[i + 1]], codes, scale, slots[i])
+        close(o[qo[i]:qo[i + 1]], want, tol, f"len {lens[i]}")
+        lse_close(lse[qo[i]:qo[i + 1]], wl, d, f"len {lens[i]}")
+
+
+def test_a_small_workspace_takes_fewer_partial_rows():
+    """A plan whose partial rows do not fit its workspace is made again with longer items;
+    one that fits in no way is refused."""
+    from beam_engine_amd import BatchDecodeWithPagedKVCacheWrapper
+    say("small workspace")
+    hq, hkv, d, page, dtype, n = 64, 8, 128, 16, torch.bfloat16, 9000
+    total, ptr, ind, last, slots = lists([n, 3], page, random.Random(1))
+    codes, scale = cache(total, page, hkv, d, 3)
+    q = torch.randn((2, hq, d), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    wide = BatchDecodeWithPagedKVCacheWrapper(workspace())
+    wide.plan(ptr, ind, last, hq, hkv, d, page, q_data_type=dtype, kv_data_type=F8)
+    small = BatchDecodeWithPagedKVCacheWrapper(torch.empty(wide._need(wide._info) - 512, dtype=torch.uint8, device="cuda"))
+    small.plan(ptr, ind, last, hq, hkv, d, page, q_data_type=dtype, kv_data_type=F8)
+    assert 0 < small.stats.num_part_rows < wide.stats.num_part_rows
+    for w in (wide, small):
+        o = w.run(q, codes, kv_scale=scale)
+        for i in range(2):
+            want, _, tol = attend(q[i:i + 1], codes, scale, slots[i])
+            close(o[i:i + 1], want, tol, f"rows {w.stats.num_part_rows}")
+    with pytest.raises(MemoryError):
+        tiny = BatchDecodeWithPagedKVCacheWrapper(torch.empty(2048, dtype=torch.uint8, device="cuda"))
+        tiny.plan(ptr, ind, last, hq, hkv, d, page, q_data_type=dtype, kv_data_type=F8)
+
+
+@pytest.mark.parametrize("tile_rows", [64, 128])
+def test_two_graphs_of_one_plan(tile_rows):
+    """A cascade of wide, narrow and short groups in a fixed layout, two layers captured as
+    a graph each over one workspace, replayed in turn, again after each new plan, with
+    eager work between: every replay gives its layer's result."""
+    from beam_engine_amd import MultiLevelCascadeAttentionWrapper
+    say(f"two graphs, {tile_rows} rows")
+    hq, hkv, d, page, dtype, beams = 16, 4, 128, 16, torch.bfloat16, 40
+    w = MultiLevelCascadeAttentionWrapper(2, workspace())
+    w.use_fixed_layout(1024, beams, 1024, beams, 4096, beams, tile_rows)
+    r = random.Random(2)
+    pools = [cache(410, page, hkv, d, 10 + l, spread=3) for l in range(2)]
+    q = torch.zeros((beams, hq, d), dtype=dtype, device="cuda")
+    outs = [torch.zeros_like(q) for _ in range(2)]
+
+    def plan(prefix, tails, groups):
+        total, ptr, ind, last, slots = lists([prefix] * groups + tails, page, r)
+        assert total <= 410
+        cut = ptr[groups]
+        edge = [i * beams // groups for i in range(groups + 1)]
+        w.plan([edge, list(range(beams + 1))], [ptr[:groups + 1], [p - cut for p in ptr[groups:]]], [ind[:cut], ind[cut:]],
+               [last[:groups], last[groups:]], hq, hkv, d, page, causal=True, q_data_type=dtype, kv_data_type=F8)
+        return [slots[max(g for g in range(groups) if edge[g] <= b)] + slots[groups + b] for b in range(beams)]
+
+    def run(layer):
+        w.run(q, pools[layer][0], kv_scale=pools[layer][1], out=outs[layer])
+
+    plan(600, [20] * beams, 1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(0)
+        run(1)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for layer in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[layer]):
+            run(layer)
+    for turn, (prefix, tails, groups) in enumerate([(600, [20] * beams, 1), (1000, [r.randrange(0, 50) for _ in range(beams)], 2),
+                                                   (33, [150] * beams, 1), (500, [0] * beams, 10), (640, [1] * beams, 1)]):
+        where = plan(prefix, tails, groups)
+        q.copy_(torch.randn(q.shape, generator=torch.Generator(device="cuda").manual_seed(turn), device="cuda"))
+        for o in outs:
+            o.fill_(7.0)
+        for layer in (0, 1, 0):
+            graphs[layer].replay()
+            torch.cuda.synchronize()
+            got = outs[layer].clone()
+            run(layer)
+            # (random codes hold some NaN)
+            assert torch.equal(outs[layer].view(torch.int16), got.view(torch.int16)), f"turn {turn} layer {layer}"
+        for layer in (0, 1):
+            for b in (0, 1, beams // 2, beams - 1):
+                want, _, tol = attend(q[b:b + 1], *pools[layer], where[b])
+                close(outs[layer][b:b + 1], want, tol, f"turn {turn} layer {layer} beam {b}")
+
+
+@pytest.mark.parametrize("kind", ["tiles", "blocks"])
+def test_far_pages(kind):
+    """Pages behind the first 2^32 bytes of a layer."""
+    say(f"far pages, {kind}")
+    page, hq, hkv, d, dtype = 16, 32, 8, 128, torch.bfloat16
+    pages = (5 << 30) // (2 * page * hkv * d)
+    codes = torch.zeros((pages, 2, page, hkv, d), dtype=torch.uint8, device="cuda").view(F8)
+    scale = torch.zeros((pages, 2, hkv), dtype=torch.uint8, device="cuda").view(E8)
+    n = 150
+    mine = [pages - 1 - 7 * i for i in range(10)]
+    few, s = cache(10, page, hkv, d, 1, spread=2)
+    codes.view(torch.uint8)[mine], scale.view(torch.uint8)[mine] = few.view(torch.uint8), s.view(torch.uint8)
+    q = torch.randn((n, hq, d), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    w = planned(kind, [0, n], [0, 10], mine, [n - 144], hq, hkv, d, page, dtype, True)
+    o = w.run(q, codes, kv_scale=scale)
+    want, _, tol = attend(q, few, s, list(range(n)), torch.arange(n, device="cuda") + 1)
+    close(o, want, tol, "far pages")
+
+
+def test_tree_entry_points():
+    """The tree's own entry points on an 8-bit cache, which they refuse without its scales."""
+    from beam_engine_amd import KVTreeNode
+    from beam_engine_amd.fasttree import fasttree_decode, prepare_fasttree_metadata_for_paged_cache
+    say("tree entry points")
+    hq, hkv, d, page, dtype = 8, 2, 128, 16, torch.bfloat16
+    codes, scale = cache(32, page, hkv, d, 4, spread=2)
+    # a root of 40 tokens that two requests share, a tail of their own each
+    spans = [(-1, 40, [0, 1]), (0, 21, [0]), (0, 5, [1])]           # parent, own tokens, requests
+    nodes, pages = [], [[0, 1, 2], [5, 6], [9]]
+    for i, (parent, n, reqs) in enumerate(spans):
+        t = KVTreeNode()
+        t.parent, t.id, t.seqlen, t.num_children, t.requests = parent, i, n + (40 if i else 0), 0 if i else 2, reqs
+        nodes.append(t)
+    slot = [[p * page + j for p in pg for j in range(page)][:n] for pg, (_, n, _) in zip(pages, spans)]
+    paths = [slot[0] + slot[1], slot[0] + slot[2]]
+    longest = max(map(len, paths))
+    req = torch.tensor([p + [0] * (longest - len(p)) for p in paths])
+    meta = prepare_fasttree_metadata_for_paged_cache(nodes, req, 2, hq, hkv, d, page_size=page, q_data_type=dtype, kv_data_type=F8)
+    q = torch.randn((2, hq, d), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    with pytest.raises(ValueError, match="kv_scale"):
+        fasttree_decode(q, codes, None, meta)
+    o = fasttree_decode(q, codes, None, meta, kv_scale=scale)
+    for b in range(2):
+        want, _, tol = attend(q[b:b + 1], codes, scale, paths[b])
+        close(o[b:b + 1], want, tol, f"request {b}")
+
+
 # ------------------------------------------------------------------ together
 def test_written_then_attended_then_captured():
     """Prompts appended and attended, a fork, and decode steps whose append and attention

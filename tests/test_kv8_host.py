@@ -97,6 +97,37 @@ def test_plan_covers_every_token(hq, hkv, d, page):
         assert at == n
 
 
+def items_of(info, buf):
+    return buf[info.off_items:info.off_items + 8 * info.num_items].reshape(-1, 8)
+
+
+@pytest.mark.parametrize("page", [8, 16, 48])
+def test_plan_names_who_takes_an_item(page):
+    """Blocks first, one wave's items last; an item is a wave's by its rows, tokens and
+    pages; NO_BLOCKS leaves blocks to groups that no tile holds."""
+    lens = (5, 128, 129, 40, 0, 700)
+    rc, info, buf = plan(hq=8, hkv=2, page=page, lens=lens)
+    assert rc == 0 and info.num_wg == 0
+    short = [x[4] <= 128 for x in items_of(info, buf)]
+    if page % 16 == 0:
+        assert info.num_tail_items == sum(short) and all(short[len(short) - sum(short):])
+    else:
+        assert info.num_tail_items == 0
+    for flags in (_lib.BE_PLAN_KV8, _lib.BE_PLAN_KV8 | _lib.BE_PLAN_NO_BLOCKS):
+        rc, info, buf = plan(hq=130, hkv=2, page=page, lens=lens, flags=flags)
+        assert rc == 0 and info.num_wg == info.num_items and info.num_tail_items == 0 and info.tile_rows == 128
+        assert all(x[7] == x[3] // page for x in items_of(info, buf))
+
+
+def test_less_scratch_does_not_cut():
+    rows = []
+    for flags in (_lib.BE_PLAN_KV8, _lib.BE_PLAN_KV8 | _lib.BE_PLAN_LESS_SCRATCH):
+        rc, info, _ = plan(hq=64, hkv=8, lens=(9000, 3), flags=flags)
+        assert rc == 0
+        rows.append(info.num_part_rows)
+    assert rows[1] == 3 < rows[0]           # an item holds at most 4032 tokens of 16-token pages
+
+
 def test_fixed_layout_keeps_its_rows():
     caps = _lib.BePlanCaps(64, 8, 64, 8, 64, 8, 64, 0)
     rc, info, _ = plan(lens=(100, 3, 0), caps=ctypes.byref(caps))
