@@ -22,6 +22,8 @@ constexpr int kLeastExp = -100;        // (2^126 of its inverse stays finite)
 constexpr int kChunk = 16;             // entries of a workgroup, at most
 constexpr int kTile = 256;             // entries of a scan step, members of a batch beyond the chunk's
 constexpr int kMembers = kChunk + kTile;
+constexpr int kFew = 256;              // entries of a call that takes four a workgroup, at most (a scan step)
+constexpr int kFewPages = 4;           // led pages that are looked for one by one
 constexpr int kHeads = 4;               // KV heads of a pass, at most
 
 // The largest e4m3 value times a power of two that the type holds: stored values
@@ -108,7 +110,7 @@ __device__ __forceinline__ void rotate(float (&v)[2 * E], const float (&c)[2 * E
 // What bounds it: a decode step's launch is a chain of round trips (indices, rows,
 // tables, the old scale); prompts are bound by the rows' bytes.
 template <typename T, int D, int PER>
-__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 4 : D == 128 ? 3 : 2) void append_kernel(AppendArgs a) {
   constexpr int E = D / 32;
   __shared__ int32_t s_page[kChunk], s_slot[kChunk], s_lead[kChunk];   // the chunk's pages (-1: skipped), slots, which lead
   __shared__ bool s_dead[kChunk];                         // written again by a later entry of the chunk
@@ -118,7 +120,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   __shared__ int32_t m_tok[kMembers], m_slot[kMembers];   // a batch: entry, slot, led page, overwritten later
   __shared__ uint8_t m_lead[kMembers], m_dead[kMembers];
   __shared__ int32_t s_range[2], s_wave[4];               // members beyond the chunk: first, last entry; compaction
-  __shared__ int32_t s_count, s_grown;
+  __shared__ int32_t s_count, s_grown, s_extra, s_any;
+  __shared__ int32_t x_tok[kChunk], x_slot[kChunk], x_lead[kChunk], x_pos[kChunk];   // members beyond the chunk, in no order
 
   const int tid = threadIdx.x, grp = tid >> 4, u = tid & 15, lane = tid & 63, wave = tid >> 6;
   constexpr int chunk = kChunk / PER, per = PER;       // entries, and 16-lane groups of one
@@ -181,7 +184,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     }
   };
   load_q(q0 + sub);                                    // (hq is 0 without a rotation)
-  constexpr int U = PER == 1 ? 8 : 4;                  // ids of a thread in flight (4: all of 1024 entries)
+  constexpr int U = PER == 1 ? 8 : 1;                  // ids of a thread in flight (1: all of kFew entries)
   int ids[U];
   auto load_ids = [&](int j0) {
 #pragma unroll
@@ -204,6 +207,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     s_first[tid] = a.page_size;
   }
   if (tid < 2) s_range[tid] = tid == 0 ? a.n : -1;
+  if (tid == 0) s_extra = s_any = 0;
   if (tid < kHeads * kChunk * 2) (&s_amax[0][0][0])[tid] = 0;
   __syncthreads();
   // which entry of the chunk leads its page, which is written again by a later one of the
@@ -227,11 +231,17 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     s_lead[tid] = w_lead;
     s_dead[tid] = w_dead;
   }
-  // one or two led pages (prompts): looked for themselves, not by the filter
-  const uint32_t leads = (uint32_t)__ballot(lane < kChunk && w_lead == lane);
-  const int page_a = leads ? __builtin_amdgcn_readlane(w_page, __builtin_ctz(leads)) : -1;
-  const int page_b = leads & (leads - 1) ? __builtin_amdgcn_readlane(w_page, __builtin_ctz(leads & (leads - 1))) : page_a;
-  const bool few = __builtin_popcount(leads) <= 2;
+  // up to four led pages (prompts): looked for themselves, not by the filter
+  uint32_t leads = (uint32_t)__ballot(lane < kChunk && w_lead == lane);
+  const bool few = __builtin_popcount(leads) <= kFewPages, more = few && __builtin_popcount(leads) > 2;
+  int f_page[kFewPages], f_lead[kFewPages];
+#pragma unroll
+  for (int i = 0; i < kFewPages; ++i) {
+    f_lead[i] = leads ? __builtin_ctz(leads) : i > 0 ? f_lead[0] : 0;
+    f_page[i] = leads || i > 0 ? __builtin_amdgcn_readlane(w_page, f_lead[i]) : -2;
+    leads &= leads - 1;
+  }
+  if (f_page[0] < 0) f_page[0] = -2;                   // (no page at all: nothing is looked for)
   __syncthreads();
 
   // ---- entries of the led pages outside the chunk
@@ -243,20 +253,44 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   auto maybe = [&](int p) { return ((p & 32 ? f1 : f0) >> (p & 31)) & 1u; };
   for (int j0 = 0; j0 < a.n; j0 += 256 * U) {
     uint32_t hits = 0;
+    if (few) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) hits |= (few ? (uint32_t)(ids[i] == page_a) | (uint32_t)(ids[i] == page_b) : maybe(ids[i])) << i;
+      for (int i = 0; i < U; ++i) hits |= ((uint32_t)(ids[i] == f_page[0]) | (uint32_t)(ids[i] == f_page[1])) << i;
+      if (more) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) hits |= ((uint32_t)(ids[i] == f_page[2]) | (uint32_t)(ids[i] == f_page[3])) << i;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < U; ++i) hits |= maybe(ids[i]) << i;
+    }
     if (PER == 1) load_ids(j0 + 256 * U);              // the next ones', ahead of these ones' hits
     while (hits) {
       const int j = j0 + 256 * __builtin_ctz(hits) + tid;
       hits &= hits - 1;
       if (j >= a.n || (j >= c0 && j < c0 + cn)) continue;
-      const int p = a.page_idx[j], l = p >= 0 ? lead_of(p) : -1;
-      if (l < 0 || !valid(j)) continue;
+      const int p = a.page_idx[j], sl = a.slot[j];       // (one round trip)
+      const int64_t at = rope ? a.positions[j] : 0;
+      int l = -1;
+      if (few) {
+#pragma unroll
+        for (int f = 0; f < kFewPages; ++f) l = p == f_page[f] ? f_lead[f] : l;
+      } else if (p >= 0) {
+        l = lead_of(p);
+      }
+      if (l < 0 || sl < 0 || sl >= a.page_size || (rope && (at < 0 || at >= a.max_pos))) continue;
       if (j < c0) {
         s_first[l] = -1;                               // led by an earlier workgroup
       } else {
         atomicMin(&s_range[0], j);
         atomicMax(&s_range[1], j);
+        const int x = atomicAdd(&s_extra, 1);
+        if (x < kChunk) {
+          x_tok[x] = j;
+          x_slot[x] = sl;
+          x_lead[x] = l;
+          x_pos[x] = (int32_t)at;
+        }
       }
     }
   }
@@ -447,18 +481,51 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         }
   };
 
-  // ---- no entry outside the chunk belongs to its pages (a decode step, prompts that start
-  // at a chunk): the groups' own rows, which are there already
-  if (tiles == 0) {
-    const int l = s_lead[own];
-    const bool led = mine && l >= 0 && s_first[max(l, 0)] >= 0;
+  // ---- at most 16 entries outside the chunk belong to its pages (decode steps, prompts on
+  // pages of up to 16 tokens): the groups' own rows, which are there already, and one
+  // such entry a group
+  const int extra = __builtin_amdgcn_readfirstlane(s_extra);
+  if (extra <= kChunk) {
+    const int l = s_lead[own], xl = grp < extra ? x_lead[grp] : -1;
+    const bool led = mine && l >= 0 && s_first[max(l, 0)] >= 0, xled = xl >= 0 && s_first[max(xl, 0)] >= 0;
+    const int xs = xl >= 0 ? x_slot[grp] : 0, xt = xl >= 0 ? x_tok[grp] : 0;
+    if (led || xled) s_any = 1;
     __syncthreads();
-    if (led && sub == 0 && u == 0) atomicMin(&s_first[l], e_slot);
+    if (!s_any) return;
+    Pack<T, E> xk_lo[HB], xk_hi[HB], xv_lo[HB], xv_hi[HB];
+    auto load_x = [&](int h) {
+#pragma unroll
+      for (int b = 0; b < HB; ++b) {
+        if (!xled || h + b >= h1) continue;
+        const T* k = reinterpret_cast<const T*>(a.k) + (int64_t)xt * a.k_sn + (int64_t)(h + b) * a.k_sh + u * E;
+        const T* v = reinterpret_cast<const T*>(a.v) + (int64_t)xt * a.v_sn + (int64_t)(h + b) * a.v_sh + u * E;
+        xk_lo[b] = *reinterpret_cast<const Pack<T, E>*>(k);
+        xk_hi[b] = *reinterpret_cast<const Pack<T, E>*>(k + D / 2);
+        xv_lo[b] = *reinterpret_cast<const Pack<T, E>*>(v);
+        xv_hi[b] = *reinterpret_cast<const Pack<T, E>*>(v + D / 2);
+      }
+    };
+    if (extra > 0) load_x(h0);
+    float xc[2 * E], xn[2 * E];
+    if (rope && xled) tables(x_pos[grp], xc, xn);
+    if (u == 0) {
+      if (led && sub == 0) atomicMin(&s_first[l], e_slot);
+      if (xled) atomicMin(&s_first[xl], xs);
+    }
+    // (of entries with the same page and slot the last is written)
+    bool write = led && !s_dead[own], xwrite = xled;
+    for (int o = 0; o < extra; ++o) {
+      const int ol = x_lead[o], os = x_slot[o];
+      write = write && !(ol == l && os == e_slot);
+      xwrite = xwrite && !(ol == xl && os == xs && x_tok[o] > xt);
+    }
     __syncthreads();
-    const bool write = led && !s_dead[own];
     for (int h = h0; h < h1; h += HB) {
       const int nh = min(HB, h1 - h), old = old_exp(h, nh);
-      if (h > h0) load_kv(h);
+      if (h > h0) {
+        load_kv(h);
+        if (extra > 0) load_x(h);
+      }
       float xk[HB][2 * E], xv[HB][2 * E];
 #pragma unroll
       for (int b = 0; b < HB; ++b) {
@@ -475,6 +542,23 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
           take_max(l, 1, b, xv[b]);
         }
       }
+      auto x_row = [&](int sel, int b, float (&x)[2 * E]) {
+        unpack<T, E>(sel ? xv_lo[b] : xk_lo[b], x, 0);
+        unpack<T, E>(sel ? xv_hi[b] : xk_hi[b], x, E);
+        if (!sel && rope) rotate<E>(x, xc, xn);
+      };
+      if (extra > 0) {
+#pragma unroll
+        for (int b = 0; b < HB; ++b) {
+          if (!xled || b >= nh) continue;
+#pragma unroll
+          for (int sel = 0; sel < 2; ++sel) {
+            float x[2 * E];
+            x_row(sel, b, x);
+            take_max(xl, sel, b, x);
+          }
+        }
+      }
       if (tid == 0) s_grown = 0;
       __syncthreads();
       new_exp(h, nh, old);
@@ -484,6 +568,18 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         if (!write || b >= nh) continue;
         if (per == 1 || sub == 0) store(l, e_slot, 0, h + b, b, xk[b]);
         if (per == 1 || sub == 1) store(l, e_slot, 1, h + b, b, xv[b]);
+      }
+      if (extra > 0) {
+#pragma unroll
+        for (int b = 0; b < HB; ++b) {
+          if (!xwrite || b >= nh) continue;
+#pragma unroll
+          for (int sel = 0; sel < 2; ++sel) {
+            float x[2 * E];
+            x_row(sel, b, x);
+            store(xl, xs, sel, h + b, b, x);
+          }
+        }
       }
       if (s_grown) rescale(h, nh);
       __syncthreads();
@@ -543,9 +639,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       __syncthreads();
     }
   };
-  if (single && members <= 16) {
-    held(std::integral_constant<int, 1>());
-  } else if (single && members <= 32) {
+  if (single && members <= 32) {
     held(std::integral_constant<int, 2>());
   } else {
     for (int h = h0; h < h1; ++h) {
@@ -651,8 +745,9 @@ static int check_cache(const void* kv, const void* scale, int num_pages, int pag
 
 // Few entries (a decode step): four a workgroup and one KV head each, so that their rows
 // spread over the CUs; many: 16 (a page's worth), and as few shares of the heads as leave
-// every CU four workgroups.
-constexpr int kFew = 1024;
+// every CU four workgroups.  At 32 heads of 128 over 8, four / 16 a workgroup: 128 lone
+// tokens 9.0 / 12.2 us, 256 9.9 / 12.8, 512 15.5 / 15.2; prompts of 256 tokens 13.3 / 10.3,
+// of 512 22.1 / 11.2.
 template <typename T, int D>
 static void launch_per(const AppendArgs& a, dim3 grid, hipStream_t st) {
   if (a.n <= kFew) append_kernel<T, D, 4><<<grid, 256, 0, st>>>(a);
