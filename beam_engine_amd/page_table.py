@@ -87,7 +87,7 @@ class PageTable:
             _lib.check(_lib.BE_ERR_INVALID, "page pool")
         self._page_out = ctypes.c_int32(0)
         self._pending: List[Tuple[int, int, int]] = []
-        self._copy_host = self._copy_dev = self._copy_ev = None     # fork-copy lists' staging
+        self._copy_staging, self._copy_at = [None] * 4, 0           # fork-copy lists' staging: (pinned, device, event)
         self._defer = 0
         # staged fork copies (stage_copies): a device list [count, src[m], dst[m], len[m]]
         # and its pinned host twin, run by one counted launch (run_staged_copies),
@@ -241,31 +241,35 @@ class PageTable:
         if n == 0:
             return 0
         if self.device.type == "cuda":
-            # pinned staging, reused once the previous flush's copy has run
-            if self._copy_host is None or self._copy_host.shape[1] < n:
+            # pinned staging, four in turn: each reused once the copies that last read it have
+            # run, on whichever stream (with one, every flush waited for the last one's)
+            at = self._copy_at = (self._copy_at + 1) % len(self._copy_staging)
+            host, buf, ev = self._copy_staging[at] or (None, None, None)
+            if host is None or host.numel() < 3 * n:
                 cap = max(256, 2 * n)
-                self._copy_host = torch.empty((3, cap), dtype=torch.int32, pin_memory=True)
-                self._copy_dev = torch.empty((3, cap), dtype=torch.int32, device=self.device)
-                self._copy_ev = None
-            if self._copy_ev is not None:
-                self._copy_ev.synchronize()
-            self._copy_host.numpy()[:, :n] = np.asarray(todo, dtype=np.int32).T
-            dev = self._copy_dev[:, :n]
-            dev.copy_(self._copy_host[:, :n], non_blocking=True)
-            self._copy_ev = torch.cuda.Event()
-            self._copy_ev.record()
+                host = torch.empty(3 * cap, dtype=torch.int32, pin_memory=True)
+                buf, ev = torch.empty(3 * cap, dtype=torch.int32, device=self.device), torch.cuda.Event()
+                self._copy_staging[at] = (host, buf, ev)
+            else:
+                ev.synchronize()
+            host.numpy()[:3 * n].reshape(3, n)[:] = np.asarray(todo, dtype=np.int32).T
+            flat = buf[:3 * n]
+            flat.copy_(host[:3 * n], non_blocking=True)
+            dev = flat.view(3, n)
         else:
-            dev = torch.from_numpy(np.ascontiguousarray(np.asarray(todo, dtype=np.int32).T))
-        lib = _lib.load()
+            dev, ev = torch.from_numpy(np.ascontiguousarray(np.asarray(todo, dtype=np.int32).T)), None
+        src, dst, length = (dev.data_ptr() + 4 * n * i for i in range(3))
         if self.kv8:
-            self._copy_kv8(dev[0].data_ptr(), dev[1].data_ptr(), dev[2].data_ptr(), 0, len(todo), "page copy")
-            return len(todo)
-        rc = lib.be_page_copy(self.kv_pool.data_ptr(), self.layer_stride_bytes, self.layer_num,
-                              _lib.dtype_code(self.store_dtype), self.max_num_pages, self.page_size,
-                              self.head_num, self.head_dim, dev[0].data_ptr(), dev[1].data_ptr(),
-                              dev[2].data_ptr(), len(todo), self._err.data_ptr(), _lib.stream_ptr(self.device))
-        _lib.check(rc, "page copy")
-        return len(todo)
+            self._copy_kv8(src, dst, length, 0, n, "page copy")
+        else:
+            rc = self._lib.be_page_copy(self.kv_pool.data_ptr(), self.layer_stride_bytes, self.layer_num,
+                                        _lib.dtype_code(self.store_dtype), self.max_num_pages, self.page_size,
+                                        self.head_num, self.head_dim, src, dst, length, n, self._err.data_ptr(),
+                                        _lib.stream_ptr(self.device))
+            _lib.check(rc, "page copy")
+        if ev is not None:
+            ev.record(torch.cuda.current_stream(self.device))
+        return n
 
     def _copy_kv8(self, src: int, dst: int, length: int, count: int, n: int, what: str) -> None:
         """Fork copies of codes and scales (device arrays; ``count`` 0 or the device count)."""

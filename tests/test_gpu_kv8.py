@@ -263,6 +263,28 @@ def test_copies_take_codes_and_scales():
             assert all(np.array_equal(a, b) for a, b in zip(state(t, l), want[l]))
 
 
+def test_copies_in_a_row():
+    """Many lists of copies in a row, each reading what the last one wrote, from two streams
+    that wait for each other: none sees another's list."""
+    say("copies in a row")
+    t = table(40, 4, 2, 64, torch.bfloat16, seed=8)
+    want = state(t)
+    side, main = torch.cuda.Stream(), torch.cuda.current_stream()
+    for i in range(14):
+        a = [(7 * i + 3 * j) % 20 for j in range(1 + 5 * i % 11)]
+        todo = np.array([(s, 20 + (s + i) % 20 if i % 2 else (s + 1) % 20, 1 + (s + i) % 4) for s in dict.fromkeys(a)], np.int32)
+        todo = todo[[k for k in range(len(todo)) if todo[k, 1] not in todo[:, 0] and todo[k, 1] not in todo[:k, 1]]]
+        for s, d, n in todo:
+            want[0][d, :, :n] = want[0][s, :, :n]
+            want[1][d] = want[1][s]
+        with torch.cuda.stream(side if i % 3 == 0 else main):
+            t.copy_pages(todo)
+        (main if i % 3 == 0 else side).wait_stream(side if i % 3 == 0 else main)
+    torch.cuda.synchronize()
+    got = state(t)
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_values_are_exact(dtype):
     """The values, in the type (fp16 rounds what lies below its subnormal step)."""
