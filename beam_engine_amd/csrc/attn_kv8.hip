@@ -15,6 +15,19 @@
 // row lc) is half the B operand of Oᵀ += Vᵀ Pᵀ, two token sub-tiles to a product; Vᵀ is
 // read from row-major V with ds_read_b64_tr_b8, whose eight rows are the same lanes'
 // tokens of both sub-tiles.
+//
+// The products stay 16-bit: the matrix instructions that take e4m3 operands sum up to
+// 2^-12.7 of the absolute sum off (measured over 64 products, against 64 bits), where
+// these sums are to be good to fp32, and would need P in 8 bits.  So a code costs a
+// conversion (5 cycles a wave instruction for two codes of 64 lanes), which bounds the
+// tiles: 2.0 to 2.4 thousand cycles for 64 tokens x 64 rows at head_dim 128 alone on a
+// CU, of which the loads' latency is a third.  Measured, with the merge: 16 sequences of
+// up to 6000 tokens (32 heads of 128 over 8) 30 us, 3.2 TB/s of codes where a copy moves
+// 4.9; 8 x 16 beams on 4096 shared tokens + 128 own ones 36 us, 2.9 TB/s; 2 x 64 beams
+// on 32768 + 512 (64 heads over 8) 185 us, 750 TFLOP/s of the 1170 of a large 16-bit
+// matrix product; 8 x 16 beams on 1136 + up to 24 20 us, where launches, a workgroup's
+// start (its record, pages, scales and first tile are round trips in a row, 3 us) and the
+// merge (4.4 us) are most of it.
 
 #include <math.h>
 
@@ -286,6 +299,13 @@ __device__ __forceinline__ WorkItem opaque(WorkItem it) {
   return it;
 }
 
+// ================================================================== 16-row tiles
+// Items of at most 16 rows (a sequence alone, few heads a group), and all at head_dim 256,
+// where 32-row tiles would not leave two workgroups a CU their registers.  Two waves share
+// a row tile's tokens while there are at most two row tiles, each with a softmax of its
+// own, joined in LDS at the end; with one row tile the other two take half the output's
+// columns (and the same scores).  (16 sequences of up to 6000 tokens: 30 us, bound by the
+// codes' bytes.)
 template <typename T, int D, int RT, int PG, bool QUADS>
 __device__ __forceinline__ void tile_item(const AttnArgs& a, const WorkItem& item, int kvh, TileShared<D>& sh) {
   const WorkItem it = opaque(item);
@@ -552,7 +572,9 @@ __device__ __forceinline__ int swz32(int r) {
 // waves share a row tile's tokens (and with one row tile two its columns).  The C layout
 // of a 32-token Sᵀ block (lane l: row l % 32, tokens 8 (i / 4) + 4 (l / 32) + i % 4) is,
 // eight registers at a time, the B operand of Oᵀ += Vᵀ Pᵀ over the token order that the
-// transposed V reads follow.
+// transposed V reads follow.  The reference of a row's softmax follows its maximum only
+// beyond 2^8, so most tiles rescale nothing.  Against 16-row tiles for the same items:
+// 4096-token prefixes of 64 rows 203 -> 178 us over four layers.
 template <typename T, int D, int RT, int PG, bool QUADS>
 __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& item, int kvh, TileShared<D>& sh) {
   const WorkItem it = opaque(item);
@@ -799,7 +821,8 @@ __device__ __forceinline__ void tile32_item(const AttnArgs& a, const WorkItem& i
 // each wave of a workgroup takes an item of its own, in steps of 16 tokens through its
 // share of the stages (as many steps in flight as the others have tiles), with no barrier.
 // Four such items would otherwise be four workgroups that start, wait and end for a tile
-// or two each.  All of a step's tokens lie in one page, so its scales are scalars.
+// or two each: 8 x 16 beams with tails of up to 24 tokens 200 -> 186 us over 8 layers.
+// All of a step's tokens lie in one page, so its scales are scalars.
 template <typename T, int D>
 __device__ __forceinline__ void wave_item(const AttnArgs& a, const WorkItem& item, int kvh, TileShared<D>& sh, int w) {
   const WorkItem it = opaque(item);
@@ -1018,7 +1041,10 @@ __device__ __forceinline__ int swz16(int r) {
 // is turned into 16-bit values once, on its way into LDS: each thread loads its share
 // of the next tile's codes into registers while the current one is computed, converts
 // it and writes it to the other stage; one barrier a tile.  K is converted relative to
-// the item's largest K scale, which the softmax's scale takes back.
+// the item's largest K scale, which the softmax's scale takes back.  8 prompts of 1024
+// tokens, 32 heads of 128 over 8: 102 us, 670 TFLOP/s with the masked halves of the
+// diagonal tiles as work not done (the tiles above take 107 to 111 for the same); bound by the
+// matrix instructions' waits for LDS and for the next tile's conversion.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void attn_kv8_block_kernel(AttnArgs a, int n_items) {
   constexpr int KS = D / 16;                         // QK contraction steps
