@@ -243,10 +243,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : D == 128 ? 3 : 2) void append_ke
 #pragma unroll
   for (int i = 0; i < kFewPages; ++i) {
     f_lead[i] = leads ? __builtin_ctz(leads) : i > 0 ? f_lead[0] : 0;
-    f_page[i] = leads || i > 0 ? __builtin_amdgcn_readlane(w_page, f_lead[i]) : -2;
+    f_page[i] = leads ? __builtin_amdgcn_readlane(w_page, f_lead[i]) : i > 0 ? f_page[0] : -1;   // (-1: no page at all)
     leads &= leads - 1;
   }
-  if (f_page[0] < 0) f_page[0] = -2;                   // (no page at all: nothing is looked for)
   __syncthreads();
 
   // ---- entries of the led pages outside the chunk
@@ -283,7 +282,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : D == 128 ? 3 : 2) void append_ke
       } else if (p >= 0) {
         l = lead_of(p);
       }
-      if (l < 0 || sl < 0 || sl >= a.page_size || (rope && (at < 0 || at >= a.max_pos))) continue;
+      if (p < 0 || l < 0 || sl < 0 || sl >= a.page_size || (rope && (at < 0 || at >= a.max_pos))) continue;
       if (j < c0) {
         s_first[l] = -1;                               // led by an earlier workgroup
       } else {

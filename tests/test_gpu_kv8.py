@@ -205,6 +205,29 @@ def test_append_skips_what_is_out_of_range():
     assert torch.equal(q[1].cpu(), qkv[1, :hq * 128].reshape(hq, 128))
 
 
+@pytest.mark.parametrize("n", [90, 700])
+@pytest.mark.parametrize("bad", [-1, -2, 12])
+def test_append_skips_whole_runs(n, bad):
+    """Workgroups all of whose entries are out of range, with entries of the same page
+    number before and behind them: nothing is written for any."""
+    say(f"append runs of page {bad}, {n} entries")
+    t = table(14, 8, 2, 64, torch.bfloat16, seed=4)
+    t.max_num_pages = 12                                    # two pages behind the pool that is named
+    codes, scale = state(t)
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn((n, 2, 64), generator=g).to(torch.bfloat16) for _ in range(2))
+    pages = [1 + i // 8 if i < 32 else 5 + i % 3 if i % 40 == 39 else bad for i in range(n)]
+    slots = [i % 8 for i in range(n)]
+    t.write_blocks_vectorized(0, i32(pages), k.cuda(), v.cuda(), i32(slots))
+    with pytest.raises(ValueError, match=f"{sum(p == bad for p in pages)} KV append"):
+        t.check_errors()
+    good = [i for i in range(n) if pages[i] != bad]
+    kv8.append(codes, scale, [pages[i] for i in good], [slots[i] for i in good], k.float().numpy()[good], v.float().numpy()[good], "bfloat16")
+    got = state(t)
+    assert np.array_equal(got[1], scale)
+    same_codes(got[0], codes)
+
+
 def test_append_takes_any_layout_and_stream():
     """Strided and unaligned keys, int64 indices, nothing to write, another stream."""
     say("append layouts and streams")
