@@ -300,6 +300,8 @@ static Kv8Cut kv8_cut(const std::vector<Group>& groups, const Vis& vis, const Ca
       }
     }
     if (qt.empty()) return Kv8Cut{rows_cap, kTile, 0};
+    // (no group has rows for blocks: the same tiles again)
+    if (best.rows_cap && std::none_of(qt.begin(), qt.end(), [](const Tile& x) { return x.rows > 64; })) continue;
     int64_t last = 0;
     for (int64_t n = 1; n <= 1024; n = n < 8 ? n + 1 : n * 9 / 8) {
       const int64_t c = ceil_div(longest, n);
