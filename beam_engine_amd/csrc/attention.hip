@@ -254,10 +254,10 @@ struct Kv8Cut {
   double us;
 };
 // Microseconds on MI355X at head_dim 128 (kv8_scale for others), fitted to 280 timed cuts
-// of 16 shapes: a 64-token tile of a CU's share and the same for a workgroup that has
+// of 16 shapes, checked on 288 of 22: a 64-token tile of a CU's share and the same for a workgroup that has
 // the CU to itself, a workgroup's start and end as the CU's time; [0] up to 64 rows,
-// [1] blocks.  The cuts they choose are 2 % behind the fastest on average, 11 % at worst;
-// a fixed chunk of 512 tokens is 11 % behind on average and 67 % at worst.  Blocks take
+// [1] blocks.  The cuts they choose are 2 % behind the fastest on average, 12 % at worst;
+// a fixed chunk of 512 tokens is 21 % behind on average and 69 % at worst.  Blocks take
 // 97 us against 104 (8 prompts of 1024 tokens, 32 heads of 128 over 8) and 61 against 70
 // (4 x 128 tokens onto 4096), but 219 against 178 where 512 rows share a prefix of 32768
 // tokens (64 heads over 8) and 51 against 39 at 4096: there the tiles' workgroups, three
