@@ -345,6 +345,8 @@ class _PagedPlanner:
         lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if return_lse else None
         stream = _lib.raw_stream(q)
         if kv8:
+            if n == 0:                # (an empty tensor has no address)
+                return (out, lse) if return_lse else out
             args = (ctypes.byref(info), self._plan_dev.data_ptr(), _lib.ptr(self._partials), qp, sn, sh, kv.data_ptr(),
                     kv_scale.data_ptr(), op, on, oh, _lib.ptr(lse), self._sm_scale)
             if torch._C._cuda_getDevice() != dev:

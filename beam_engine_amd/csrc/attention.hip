@@ -31,8 +31,9 @@ struct MergeArgs {
   void* out;
   int64_t o_sn, o_sh;
   float* out_lse;
-  const int32_t* live;         // fixed layout: live entry count (surplus workgroups exit)
-  int hq;
+  const int32_t* zero_q;       // queries without keys, behind the first num_merge workgroups
+  const int32_t *live, *live_zero;   // fixed layout: live entry counts (surplus workgroups exit)
+  int hq, num_merge;
 };
 
 // ================================================================== VALU kernel
@@ -182,12 +183,19 @@ constexpr int kMergeBatch = 8;
 template <typename T, int D>
 __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
   constexpr int C4 = D / 4;                       // float4 columns per head
-  if (a.live && (int)blockIdx.x >= *a.live) return;
+  const bool zero = (int)blockIdx.x >= a.num_merge;
+  const int x = zero ? (int)blockIdx.x - a.num_merge : (int)blockIdx.x;
+  const int32_t* live = zero ? a.live_zero : a.live;
+  if (live && x >= *live) return;
   const int i = blockIdx.y * 256 + threadIdx.x, h = i / C4, c = i - h * C4;
   const int hq = a.hq;
   if (h >= hq) return;
-  const int qi = a.merge_q[blockIdx.x];
-  const int b = a.merge_ptr[blockIdx.x], e = a.merge_ptr[blockIdx.x + 1];
+  const int qi = (zero ? a.zero_q : a.merge_q)[x];
+  int b = 0, e = 0;
+  if (!zero) {
+    b = a.merge_ptr[x];
+    e = a.merge_ptr[x + 1];
+  }
   float M = -INFINITY, z = 0.f;
   v4f acc = {0.f, 0.f, 0.f, 0.f};
   for (int r0 = b; r0 < e; r0 += kMergeBatch) {
@@ -195,8 +203,11 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
     v4f o[kMergeBatch];
 #pragma unroll
     for (int u = 0; u < kMergeBatch; ++u) {
-      const int64_t row = (int64_t)a.merge_rows[min(r0 + u, e - 1)] * hq + h;
-      l[u] = r0 + u < e ? a.part_lse[row] : -INFINITY;
+      l[u] = -INFINITY;
+      o[u] = v4f{0.f, 0.f, 0.f, 0.f};
+      if (r0 + u >= e) continue;
+      const int64_t row = (int64_t)a.merge_rows[r0 + u] * hq + h;
+      l[u] = a.part_lse[row];
       o[u] = *reinterpret_cast<const v4f*>(a.part_o + row * D + 4 * c);
     }
     float m = M;
@@ -895,19 +906,19 @@ int attn_run(const be_attn_plan_info* info, const int32_t* plan, void* partials,
   m.part_o = a.part_o; m.part_lse = a.part_lse;
   m.merge_rows = plan + info->off_merge_rows;
   m.out = out; m.o_sn = o_sn; m.o_sh = o_sh; m.out_lse = lse; m.hq = info->num_qo_heads;
-  for (int pass = 0; pass < 2; ++pass) {
-    // pass 0: split-K merge (separate-merge plans); pass 1: queries without keys
-    const int count = pass == 0 ? (info->fused_merge ? 0 : info->grid_merge) : info->grid_zero;
-    if (count == 0) continue;
-    m.live = info->static_layout ? plan + (pass == 0 ? kHdrMerge : kHdrZero) : nullptr;
-    m.merge_q = plan + (pass == 0 ? info->off_merge_q : info->off_zero_q);
-    m.merge_ptr = plan + (pass == 0 ? info->off_merge_ptr : info->off_zero_ptr);
-    switch (info->dtype) {
-      case BE_F32: rc = launch_merge<float>(info, m, count, st); break;
-      case BE_F16: rc = launch_merge<f16_t>(info, m, count, st); break;
-      case BE_BF16: rc = launch_merge<bf16_t>(info, m, count, st); break;
-    }
-    if (rc) return rc;
+  // one launch: the split-K merge (separate-merge plans), then the queries without keys
+  m.num_merge = info->fused_merge ? 0 : info->grid_merge;
+  const int count = m.num_merge + info->grid_zero;
+  if (count == 0) return rc;
+  m.live = info->static_layout ? plan + kHdrMerge : nullptr;
+  m.live_zero = info->static_layout ? plan + kHdrZero : nullptr;
+  m.merge_q = plan + info->off_merge_q;
+  m.merge_ptr = plan + info->off_merge_ptr;
+  m.zero_q = plan + info->off_zero_q;
+  switch (info->dtype) {
+    case BE_F32: rc = launch_merge<float>(info, m, count, st); break;
+    case BE_F16: rc = launch_merge<f16_t>(info, m, count, st); break;
+    case BE_BF16: rc = launch_merge<bf16_t>(info, m, count, st); break;
   }
   return rc;
 }

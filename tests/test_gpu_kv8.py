@@ -712,6 +712,19 @@ def test_waves_of_short_items(hq, hkv, d, dtype, page):
         lse_close(lse[qo[i]:qo[i + 1]], wl, d, f"len {lens[i]}")
 
 
+def test_nothing_to_attend():
+    """No queries at all, and queries without any key: zeros and an lse of -inf."""
+    from beam_engine_amd import BatchDecodeWithPagedKVCacheWrapper
+    say("nothing to attend")
+    hq, hkv, d, page, dtype = 8, 2, 128, 16, torch.bfloat16
+    codes, scale = cache(4, page, hkv, d, 1)
+    w = BatchDecodeWithPagedKVCacheWrapper(workspace())
+    for n in (0, 3):
+        w.plan([0] * (n + 1), [], [0] * n, hq, hkv, d, page, q_data_type=dtype, kv_data_type=F8)
+        o, lse = w.run(torch.ones((n, hq, d), dtype=dtype, device="cuda"), codes, kv_scale=scale, return_lse=True)
+        assert o.shape == (n, hq, d) and not o.any() and bool(torch.isneginf(lse).all())
+
+
 def test_a_small_workspace_takes_fewer_partial_rows():
     """A plan whose partial rows do not fit its workspace is made again with longer items;
     one that fits in no way is refused."""

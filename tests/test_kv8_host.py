@@ -198,3 +198,13 @@ def test_runs_name_their_cache():
     rc, other, _ = plan(flags=0)
     assert rc == 0
     assert lib.be_attn_run_kv8(ctypes.byref(other), one, one, one, 1024, 128, one, one, one, 1024, 128, *tail) == _lib.BE_ERR_INVALID
+
+
+def test_a_launch_has_its_limit():
+    """Work items x KV heads beyond a grid are refused (nothing is launched)."""
+    lib = _lib.load()
+    _, info, _ = plan(hq=8, hkv=8)
+    one = 1 << 20
+    info.grid_items = 1 << 21
+    rc = lib.be_attn_run_kv8(ctypes.byref(info), one, one, one, 1024, 128, one, one, one, 1024, 128, None, 1.0, 3, None)
+    assert rc == _lib.BE_ERR_INVALID and b"exceed a launch" in lib.be_last_error()
