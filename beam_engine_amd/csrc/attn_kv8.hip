@@ -18,7 +18,7 @@
 //
 // Scores, the softmax's maxima and sums, the outputs' sums and split partials are fp32.
 // Rounded once each, as the matrix instructions take them: a weight P to 16 bits (half a
-// step, 2^-9 of it in bf16, 2^-12 in fp16; its sum is taken before), which is what the
+// step, up to 2^-8 of it in bf16, 2^-11 in fp16; its sum is taken before), which is what the
 // error against 64 bits consists of (2.3e-3 and 2.5e-4 in the 2-norm, of which the
 // output's own rounding is 1.7e-3 and 2.1e-4).
 //
