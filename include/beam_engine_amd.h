@@ -236,7 +236,8 @@ typedef struct be_level {
 #define BE_PLAN_NO_TAIL_ROLE 2048 /* streaming kernel: tail chunks always in the merge kernel */
 #define BE_PLAN_NO_BLOCKS 4096   /* causal groups stay on the streaming kernel where it applies
                                     (by default plans with many query rows run as 128-row
-                                    blocks, whose split keys take fp32 partial rows)         */
+                                    blocks, whose split keys take fp32 partial rows);
+                                    8-bit caches: items of at most 64 rows, where a GQA group fits */
 #define BE_PLAN_LESS_SCRATCH 8192 /* for a workspace that the default plan does not fit: causal
                                     groups on the streaming kernel where it applies (16-bit
                                     partials) and elsewhere cut as decode groups are, fp32
